@@ -9,7 +9,7 @@ module's ``own`` is true.  ``exact`` computes the same results in 64 bits.
 A page of the 4-bit cache holds, for each key/value head, ``page_tokens`` key
 rows and value rows of head_dim / 2 bytes (channel 2i in the low nibble of
 byte i), then a (scale, minimum) pair of float16 for each key row and each
-value row; a code c stands for minimum + scale * c.
+value row; a code c stands for minimum + scale * c, where scale is the row's range times 1 / 15 in 32 bits.
 """
 import math
 
@@ -170,7 +170,7 @@ def quantized(x):
     """Rows [..., head_dim] in 32 bits -> codes (uint8) and the float16 pair (scale, minimum) of each row."""
     low, high = x.amin(-1), x.amax(-1)
     minimum = low.to(torch.float16)
-    scale = ((high - minimum.float()) / 15.0).to(torch.float16)
+    scale = ((high - minimum.float()) * (1.0 / 15.0)).to(torch.float16)
     t = (x.double() - minimum.double().unsqueeze(-1)) / scale.double().unsqueeze(-1)
     codes = torch.round(t).clamp(0, 15)
     return torch.where(scale.unsqueeze(-1) > 0, codes, torch.zeros_like(codes)).to(torch.uint8), torch.stack(
@@ -536,7 +536,7 @@ def exact_append(s):
     back = []
     for x in (s["k"].double(), s["v"].double()):
         low = x.min(-1, keepdim=True).values.half().double()
-        step = ((x.max(-1, keepdim=True).values - low).float() / 15).half().double()
+        step = ((x.max(-1, keepdim=True).values - low).float() * (1.0 / 15.0)).half().double()
         code = torch.where(step > 0, torch.round((x - low) / step.clamp(min=1e-30)), torch.zeros_like(x))
         back.append(low + step * code.clamp(0, 15))
     return tuple(back)
