@@ -316,6 +316,106 @@ mc_status mc_q8_linear_noalloc(const float *x, int32_t m, int32_t k, const int8_
  * current device (non-finite quantizer input, wait timeout); synchronizes. */
 mc_status mc_op_status(uint32_t *status_bits);
 
+/* ---- decode-step operators --------------------------------------------------
+ * Attention over a cache held in 4 bits, attention to an encoder's states and
+ * sampling of the next token, for callers that run a decoder of their own.
+ * The reference has none of them: its engine keeps f32 caches (crates/
+ * marian-cpu/src/q8_engine.rs:511-574) and picks the argmax (:749-790).
+ *
+ * Every pointer in the structs below is a device pointer of the current
+ * device unless it says otherwise, arrays are dense unless they come with
+ * strides, and strides count elements.  The struct itself is read during the
+ * call.  The calls are asynchronous on `stream` (a cudaStream_t of the current
+ * device, 0 = default), allocate nothing and can be captured in a CUDA graph
+ * (the first call on a device sets up the status word: make one before any
+ * capture).  Arguments that can be seen to be wrong on the host return
+ * MC_INVALID_INPUT before anything is launched.  Lengths, starts and page ids
+ * live on the device; those that fall outside the stated bounds set the
+ * index bit read by mc_op_status, and their sequence (or, for a page id, that
+ * page's keys) is left out. */
+
+/* Element type of rows and logits. */
+typedef enum { MC_F32 = 0, MC_F16 = 1, MC_BF16 = 2 } mc_dtype;
+
+/* A paged key/value cache in 4 bits.  Each cached row of head_dim values x
+ * (one token, one key/value head, key or value) is held as
+ *   minimum = f16(min x),  scale = f16(f32(max x - minimum) * f32(1 / 15)),
+ *   code    = clamp(round((x - minimum) / scale), 0, 15)   (ties to even;
+ *             0 when scale is 0),
+ * and stands for minimum + scale * code.  A page holds page_tokens tokens of
+ * every key/value head; for each head, in this order: the key rows' codes
+ * [page_tokens][head_dim / 2] bytes (channel 2i in the low nibble of byte i,
+ * 2i + 1 in the high one), the value rows' codes, the key rows' (scale,
+ * minimum) f16 pairs [page_tokens][2], the value rows' pairs.  Position p of
+ * sequence b is slot p % page_tokens of page page_table[b][p / page_tokens]. */
+typedef struct {
+    void *pages;                 /* n_pages * mc_kv4_page_bytes(...) bytes, 16-byte aligned */
+    const int32_t *page_table;   /* [batch][pages_per_seq] page ids */
+    int64_t n_pages;
+    int32_t page_tokens;         /* 8, 16 or 32 */
+    int32_t kv_heads;            /* >= 1 */
+    int32_t head_dim;            /* a multiple of 16, 16..128 */
+    int32_t batch;               /* sequences, >= 0 */
+    int32_t pages_per_seq;       /* >= 1; pages_per_seq * page_tokens < 2^31 */
+} mc_kv4_cache;
+
+/* Bytes of one page; 0 for a shape the cache does not have. */
+uint64_t mc_kv4_page_bytes(int32_t page_tokens, int32_t kv_heads, int32_t head_dim);
+
+/* Key and value rows to put into a cache or to read back from it: rows
+ * start[b] + 0..count[b]-1 of k and v ([rows][kv_heads][head_dim] by their
+ * strides) belong to positions first[b] + 0..count[b]-1 of sequence b. */
+typedef struct {
+    void *k, *v;                 /* 16-byte aligned; strides * element size multiples of 16 */
+    const int32_t *start, *count, *first;  /* [batch] */
+    int64_t rows;
+    int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int32_t dtype;               /* mc_dtype of k and v */
+    int32_t max_count;           /* no count[b] is above it */
+} mc_kv4_rows;
+
+/* Quantizes rows into the cache (k and v are read).  A row with a NaN or an
+ * infinity, or whose minimum or scale f16 cannot hold, is stored as zeros
+ * and sets the non-finite bit.  Positions must belong to one sequence only:
+ * two sequences whose tables share a page must not both write its slots in
+ * one call. */
+mc_status mc_kv4_append(const mc_kv4_cache *cache, const mc_kv4_rows *rows, void *stream);
+
+/* The values that the cache holds at those positions (k and v are written,
+ * rounded to their type; their rows must not overlap one another). */
+mc_status mc_kv4_read(const mc_kv4_cache *cache, const mc_kv4_rows *rows, void *stream);
+
+/* Attention of q_len[b] queries of sequence b (rows q_start[b] + i of q and
+ * out, [q_rows][heads][head_dim] by their strides) over the cache's first
+ * kv_len[b] positions: out = sum_j w_j v_j / sum_j w_j, w_j = exp(scale *
+ * q . k_j), query head h with key/value head h / (heads / kv_heads).
+ * causal != 0: query i sees the positions below kv_len[b] - (q_len[b] - 1 -
+ * i), so the queries are the last q_len[b] positions; causal == 0: all of
+ * them.  A query that sees nothing gets zeros and lse -inf.  lse (nullable,
+ * [q_rows][heads]) receives ln sum_j w_j.  Rows outside every sequence are
+ * left as they were; q ranges must not overlap.  16-bit types: the weights
+ * are rounded to 11 bits before they meet the values; f32: to 22. */
+typedef struct {
+    const void *q;               /* 16-byte aligned; strides as in mc_kv4_rows */
+    void *out;                   /* may not overlap q */
+    float *lse;
+    const int32_t *q_start, *q_len, *kv_len;  /* [batch] */
+    void *workspace;             /* 16-byte aligned; calls that overlap on the GPU need their own */
+    uint64_t workspace_bytes;    /* at least mc_kv4_attention_workspace(...) */
+    int64_t q_rows;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    int32_t dtype;               /* mc_dtype of q and out */
+    int32_t heads;               /* a multiple of the cache's kv_heads */
+    int32_t max_q_len, max_kv_len;  /* no q_len[b] / kv_len[b] is above them */
+    int32_t causal;
+    float scale;                 /* finite, commonly 1 / sqrt(head_dim) */
+} mc_kv4_attention_args;
+
+/* Workspace bytes for a call with these sizes (pointers are not looked at);
+ * 0 when none is needed. */
+uint64_t mc_kv4_attention_workspace(const mc_kv4_cache *cache, const mc_kv4_attention_args *args);
+mc_status mc_kv4_attention(const mc_kv4_cache *cache, const mc_kv4_attention_args *args, void *stream);
+
 /* ---- long-text splitting ----------------------------------------------------
  * Replaces marian_core::segment_text (crates/marian-core/src/segmenter.rs:
  * 122-197), which the reference's backends call before tokenizing a request

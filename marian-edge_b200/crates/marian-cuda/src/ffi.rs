@@ -91,6 +91,65 @@ pub type mc_piece_count_fn = unsafe extern "C" fn(
 
 pub const MC_Q8_LINEAR_NOALLOC_MAX_ACTIVATIONS: u32 = 8 * 1024 * 1024;
 
+// mc_dtype
+pub const MC_F32: i32 = 0;
+pub const MC_F16: i32 = 1;
+pub const MC_BF16: i32 = 2;
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct mc_kv4_cache {
+    pub pages: *mut c_void,
+    pub page_table: *const i32,
+    pub n_pages: i64,
+    pub page_tokens: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub batch: i32,
+    pub pages_per_seq: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct mc_kv4_rows {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub start: *const i32,
+    pub count: *const i32,
+    pub first: *const i32,
+    pub rows: i64,
+    pub k_row_stride: i64,
+    pub k_head_stride: i64,
+    pub v_row_stride: i64,
+    pub v_head_stride: i64,
+    pub dtype: i32,
+    pub max_count: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct mc_kv4_attention_args {
+    pub q: *const c_void,
+    pub out: *mut c_void,
+    pub lse: *mut f32,
+    pub q_start: *const i32,
+    pub q_len: *const i32,
+    pub kv_len: *const i32,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: u64,
+    pub q_rows: i64,
+    pub q_row_stride: i64,
+    pub q_head_stride: i64,
+    pub out_row_stride: i64,
+    pub out_head_stride: i64,
+    pub dtype: i32,
+    pub heads: i32,
+    pub max_q_len: i32,
+    pub max_kv_len: i32,
+    pub causal: i32,
+    pub scale: f32,
+}
+
 // Kernel classes of mc_profile_read.
 pub const MC_KERNEL_KINDS: i32 = 14;
 
@@ -246,6 +305,26 @@ unsafe extern "C" {
         status_bits: *mut u32,
     ) -> mc_status;
     pub fn mc_op_status(status_bits: *mut u32) -> mc_status;
+    pub fn mc_kv4_page_bytes(page_tokens: i32, kv_heads: i32, head_dim: i32) -> u64;
+    pub fn mc_kv4_append(
+        cache: *const mc_kv4_cache,
+        rows: *const mc_kv4_rows,
+        stream: *mut c_void,
+    ) -> mc_status;
+    pub fn mc_kv4_read(
+        cache: *const mc_kv4_cache,
+        rows: *const mc_kv4_rows,
+        stream: *mut c_void,
+    ) -> mc_status;
+    pub fn mc_kv4_attention_workspace(
+        cache: *const mc_kv4_cache,
+        args: *const mc_kv4_attention_args,
+    ) -> u64;
+    pub fn mc_kv4_attention(
+        cache: *const mc_kv4_cache,
+        args: *const mc_kv4_attention_args,
+        stream: *mut c_void,
+    ) -> mc_status;
     pub fn mc_segment_text(
         text: *const c_char,
         len: usize,

@@ -5,6 +5,7 @@
 
 #include <cmath>
 
+#include "decode_ops.cuh"
 #include "kernels.cuh"
 #include "linear_ln.cuh"
 #include "marian_cuda.h"
@@ -15,8 +16,10 @@ namespace {
 std::mutex g_status_mutex;
 uint32_t* g_status[64] = {nullptr};
 
+}  // namespace
+
 // The operator API's per-device status word (allocated once per device).
-uint32_t* op_status_word() {
+uint32_t* mc::op_status_word() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
   std::lock_guard<std::mutex> lock(g_status_mutex);
@@ -29,7 +32,7 @@ uint32_t* op_status_word() {
   return g_status[dev];
 }
 
-}  // namespace
+using mc::op_status_word;
 
 extern "C" mc_status mc_q8_gemm(const int8_t* a, const int8_t* w, int32_t m, int32_t n, int32_t k,
                                 const float* row_scale, const float* col_scale, const float* bias,

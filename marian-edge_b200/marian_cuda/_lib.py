@@ -21,6 +21,7 @@ EXPORTS = [
     "mc_profile_read", "mc_launch_count", "mc_q8_linear", "mc_q8_linear_noalloc", "mc_q8_linear_ln", "mc_load_shortlist",
     "mc_segment_text", "mc_timeline", "mc_timeline_read", "mc_inspect_marian_bin",
     "mc_encode_token_ids", "mc_replay",
+    "mc_kv4_page_bytes", "mc_kv4_append", "mc_kv4_read", "mc_kv4_attention_workspace", "mc_kv4_attention",
 ]
 
 # MC_Q8_LINEAR_NOALLOC_MAX_ACTIVATIONS in include/marian_cuda.h
@@ -65,6 +66,32 @@ class ModelReport(C.Structure):
                 ("decoder_output_alpha", C.c_float), ("engine_graph", C.c_int32),
                 ("decoder_kind", C.c_int32), ("dim", C.c_int32), ("heads", C.c_int32),
                 ("encoder_layers", C.c_int32), ("decoder_layers", C.c_int32)]
+
+
+# mc_dtype
+MC_F32, MC_F16, MC_BF16 = range(3)
+
+
+class Kv4Cache(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("page_table", C.c_void_p), ("n_pages", C.c_int64),
+                ("page_tokens", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("batch", C.c_int32), ("pages_per_seq", C.c_int32)]
+
+
+class Kv4Rows(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("start", C.c_void_p), ("count", C.c_void_p),
+                ("first", C.c_void_p), ("rows", C.c_int64), ("k_row_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("v_row_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("dtype", C.c_int32), ("max_count", C.c_int32)]
+
+
+class Kv4AttentionArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("q_start", C.c_void_p),
+                ("q_len", C.c_void_p), ("kv_len", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64), ("q_rows", C.c_int64), ("q_row_stride", C.c_int64),
+                ("q_head_stride", C.c_int64), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("dtype", C.c_int32), ("heads", C.c_int32), ("max_q_len", C.c_int32), ("max_kv_len", C.c_int32),
+                ("causal", C.c_int32), ("scale", C.c_float)]
 
 
 class MarianCudaError(RuntimeError):
@@ -126,6 +153,13 @@ def load(build_if_missing: bool = True):
     lib.mc_encode_token_ids.argtypes = [vp, vp, sz, vp, u32, vp]
     lib.mc_replay.argtypes = [vp, vp, sz, vp, u32, vp, vp, vp, vp]
     lib.mc_inspect_marian_bin.argtypes = [C.c_char_p, sz, C.POINTER(ModelReport), C.c_char_p, sz]
+    lib.mc_kv4_page_bytes.argtypes = [i32, i32, i32]
+    lib.mc_kv4_page_bytes.restype = u64
+    lib.mc_kv4_append.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4Rows), vp]
+    lib.mc_kv4_read.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4Rows), vp]
+    lib.mc_kv4_attention_workspace.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionArgs)]
+    lib.mc_kv4_attention_workspace.restype = u64
+    lib.mc_kv4_attention.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionArgs), vp]
     lib.mc_launch_count.argtypes = [vp]
     lib.mc_launch_count.restype = u64
     _lib = lib
