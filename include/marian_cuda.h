@@ -416,6 +416,41 @@ typedef struct {
 uint64_t mc_kv4_attention_workspace(const mc_kv4_cache *cache, const mc_kv4_attention_args *args);
 mc_status mc_kv4_attention(const mc_kv4_cache *cache, const mc_kv4_attention_args *args, void *stream);
 
+/* The next token of each row from its logits and one given random number.
+ * With the row's ids ordered by logit (largest first, equal logits by id) and
+ * w = exp((logit - largest) / temperature):
+ *   A = the first top_k ids (all of them for top_k <= 0),
+ *   B = the shortest prefix of A with sum w >= top_p * sum_A w (A itself for
+ *       top_p >= 1 or NaN, its first id for top_p <= 0),
+ *   C = the ids of B with w >= min_p (B itself for min_p <= 0 or NaN; above 1
+ *       it counts as 1),
+ *   tokens[row] = the first id of C, ascending, at which the running sum of w
+ *       over C exceeds uniform * sum_C w, and probs[row] = its w / sum_C w.
+ * temperature 0 takes the largest logit (lowest id) with probability 1;
+ * a negative or NaN temperature gives token -1, probability 0 and the index
+ * bit.  -inf and NaN logits are never drawn (a NaN sets the non-finite bit);
+ * +inf logits share the whole probability.  A row with nothing to draw gives
+ * token -1 and probability 0.  Weights below 2^-41 count as 0.  The result
+ * does not depend on the launch: sums are whole numbers of 2^-40. */
+typedef struct {
+    const void *logits;          /* [rows][vocab], row_stride elements apart */
+    const float *temperature;    /* [rows]; NULL: 1 */
+    const int32_t *top_k;        /* [rows]; NULL: off */
+    const float *top_p;          /* [rows]; NULL: off */
+    const float *min_p;          /* [rows]; NULL: off */
+    const float *uniform;        /* [rows], in [0, 1); clamped to [0, 1], NaN counts as 0 */
+    const uint32_t *candidates;  /* NULL, or a bit per id (bit id % 32 of word id / 32): 0 = never drawn */
+    int32_t *tokens;             /* [rows] */
+    float *probs;                /* [rows]; NULL: not wanted */
+    int64_t row_stride;
+    int64_t candidates_stride;   /* words between rows; 0: every row has the same */
+    int32_t dtype;               /* mc_dtype of logits */
+    int32_t rows;
+    int32_t vocab;               /* 1..393216 */
+} mc_sample_args;
+
+mc_status mc_sample(const mc_sample_args *args, void *stream);
+
 /* ---- long-text splitting ----------------------------------------------------
  * Replaces marian_core::segment_text (crates/marian-core/src/segmenter.rs:
  * 122-197), which the reference's backends call before tokenizing a request

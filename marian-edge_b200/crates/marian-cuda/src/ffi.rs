@@ -150,6 +150,25 @@ pub struct mc_kv4_attention_args {
     pub scale: f32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct mc_sample_args {
+    pub logits: *const c_void,
+    pub temperature: *const f32,
+    pub top_k: *const i32,
+    pub top_p: *const f32,
+    pub min_p: *const f32,
+    pub uniform: *const f32,
+    pub candidates: *const u32,
+    pub tokens: *mut i32,
+    pub probs: *mut f32,
+    pub row_stride: i64,
+    pub candidates_stride: i64,
+    pub dtype: i32,
+    pub rows: i32,
+    pub vocab: i32,
+}
+
 // Kernel classes of mc_profile_read.
 pub const MC_KERNEL_KINDS: i32 = 14;
 
@@ -325,6 +344,7 @@ unsafe extern "C" {
         args: *const mc_kv4_attention_args,
         stream: *mut c_void,
     ) -> mc_status;
+    pub fn mc_sample(args: *const mc_sample_args, stream: *mut c_void) -> mc_status;
     pub fn mc_segment_text(
         text: *const c_char,
         len: usize,

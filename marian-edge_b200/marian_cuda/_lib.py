@@ -22,6 +22,7 @@ EXPORTS = [
     "mc_segment_text", "mc_timeline", "mc_timeline_read", "mc_inspect_marian_bin",
     "mc_encode_token_ids", "mc_replay",
     "mc_kv4_page_bytes", "mc_kv4_append", "mc_kv4_read", "mc_kv4_attention_workspace", "mc_kv4_attention",
+    "mc_sample",
 ]
 
 # MC_Q8_LINEAR_NOALLOC_MAX_ACTIVATIONS in include/marian_cuda.h
@@ -94,6 +95,13 @@ class Kv4AttentionArgs(C.Structure):
                 ("causal", C.c_int32), ("scale", C.c_float)]
 
 
+class SampleArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+                ("min_p", C.c_void_p), ("uniform", C.c_void_p), ("candidates", C.c_void_p), ("tokens", C.c_void_p),
+                ("probs", C.c_void_p), ("row_stride", C.c_int64), ("candidates_stride", C.c_int64),
+                ("dtype", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32)]
+
+
 class MarianCudaError(RuntimeError):
     def __init__(self, status, message):
         super().__init__(f"{STATUS_NAMES.get(status, status)}: {message}")
@@ -160,6 +168,7 @@ def load(build_if_missing: bool = True):
     lib.mc_kv4_attention_workspace.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionArgs)]
     lib.mc_kv4_attention_workspace.restype = u64
     lib.mc_kv4_attention.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionArgs), vp]
+    lib.mc_sample.argtypes = [C.POINTER(SampleArgs), vp]
     lib.mc_launch_count.argtypes = [vp]
     lib.mc_launch_count.restype = u64
     _lib = lib
