@@ -416,6 +416,42 @@ typedef struct {
 uint64_t mc_kv4_attention_workspace(const mc_kv4_cache *cache, const mc_kv4_attention_args *args);
 mc_status mc_kv4_attention(const mc_kv4_cache *cache, const mc_kv4_attention_args *args, void *stream);
 
+/* Attention of packed queries to an encoder's states: queries q_start[b] +
+ * 0..q_len[b]-1 (rows of q and out, [q_rows][heads][head_dim] by their
+ * strides) over keys k_start[b] + 0..k_len[b]-1 (rows of k and v,
+ * [k_rows][kv_heads][head_dim]): out = sum_j w_j v_j / sum_j w_j, w_j =
+ * exp(scale * q . k_j), query head h with key/value head h / (heads /
+ * kv_heads).  Sequences may share keys (the same k_start for several
+ * translations of one source), may leave gaps (padded batches) and may have
+ * q_len 1 (a decode step).  key_mask (nullable, a byte per row of k): keys
+ * with 0 are left out, whatever they hold.  A query with no key left gets
+ * zeros and lse -inf; lse (nullable, [q_rows][heads]) receives ln sum_j w_j.
+ * Rows outside every sequence are left as they were; q ranges must not
+ * overlap.  16-bit types: the weights are rounded to the type before they
+ * meet the values; f32: products to 2^-21. */
+typedef struct {
+    const void *q, *k, *v;       /* 16-byte aligned; strides * element size multiples of 16 */
+    void *out;                   /* may not overlap q, k or v */
+    float *lse;
+    const int32_t *q_start, *q_len, *k_start, *k_len;  /* [batch] */
+    const uint8_t *key_mask;
+    void *workspace;             /* 16-byte aligned; calls that overlap on the GPU need their own */
+    uint64_t workspace_bytes;    /* at least mc_cross_attention_workspace(...) */
+    int64_t q_rows, k_rows;
+    int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride;
+    int64_t v_row_stride, v_head_stride, out_row_stride, out_head_stride;
+    int32_t dtype;               /* mc_dtype of q, k, v and out */
+    int32_t batch, heads, kv_heads;  /* heads a multiple of kv_heads */
+    int32_t head_dim;            /* a multiple of 16, 16..128 */
+    int32_t max_q_len, max_k_len;  /* no q_len[b] / k_len[b] is above them */
+    float scale;                 /* finite, commonly 1 / sqrt(head_dim) */
+} mc_cross_attention_args;
+
+/* Workspace bytes for a call with these sizes (pointers are not looked at);
+ * 0 when none is needed. */
+uint64_t mc_cross_attention_workspace(const mc_cross_attention_args *args);
+mc_status mc_cross_attention(const mc_cross_attention_args *args, void *stream);
+
 /* The next token of each row from its logits and one given random number.
  * With the row's ids ordered by logit (largest first, equal logits by id) and
  * w = exp((logit - largest) / temperature):

@@ -152,6 +152,41 @@ pub struct mc_kv4_attention_args {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct mc_cross_attention_args {
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub out: *mut c_void,
+    pub lse: *mut f32,
+    pub q_start: *const i32,
+    pub q_len: *const i32,
+    pub k_start: *const i32,
+    pub k_len: *const i32,
+    pub key_mask: *const u8,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: u64,
+    pub q_rows: i64,
+    pub k_rows: i64,
+    pub q_row_stride: i64,
+    pub q_head_stride: i64,
+    pub k_row_stride: i64,
+    pub k_head_stride: i64,
+    pub v_row_stride: i64,
+    pub v_head_stride: i64,
+    pub out_row_stride: i64,
+    pub out_head_stride: i64,
+    pub dtype: i32,
+    pub batch: i32,
+    pub heads: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub max_q_len: i32,
+    pub max_k_len: i32,
+    pub scale: f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct mc_sample_args {
     pub logits: *const c_void,
     pub temperature: *const f32,
@@ -342,6 +377,11 @@ unsafe extern "C" {
     pub fn mc_kv4_attention(
         cache: *const mc_kv4_cache,
         args: *const mc_kv4_attention_args,
+        stream: *mut c_void,
+    ) -> mc_status;
+    pub fn mc_cross_attention_workspace(args: *const mc_cross_attention_args) -> u64;
+    pub fn mc_cross_attention(
+        args: *const mc_cross_attention_args,
         stream: *mut c_void,
     ) -> mc_status;
     pub fn mc_sample(args: *const mc_sample_args, stream: *mut c_void) -> mc_status;

@@ -1,0 +1,594 @@
+// cross_attn.cu -- attention of packed queries to the states of an encoder
+// whose sequences have another length (mc_cross_attention).
+//
+// out_i = sum_j w_ij v_j / sum_j w_ij, w_ij = exp(scale q_i . k_j), over the
+// keys of the query's sequence that the mask leaves in.  One pass over the
+// keys with the running maximum and sum of each row in registers.
+#include <cstring>
+
+#include "decode_ops.cuh"
+
+namespace mc {
+namespace {
+
+constexpr uint32_t kFull = 0xFFFFFFFFu;
+constexpr int kSms = 148;
+
+struct CrossParams {
+  AttnRows rows;
+  AttnSplit split;
+  const void *k, *v;
+  long long k_rs, k_hs, v_rs, v_hs;
+  const uint8_t* mask;
+  float scale;
+  int row_tiles;
+  uint32_t* status;
+};
+
+// ---- small tiles: mma.sync ------------------------------------------------------------
+// Four warps: WR of them side by side over 16 rows each, the other 4 / WR
+// groups over parts of every key tile, so that a unit of 16 rows (a decode
+// step's) still has four warps on its keys.  Rows are (position, head of the
+// group): shared heads fill the row tile of a single position.
+//
+// 16-bit types: m16n8k16, weights rounded to the values' type after a shift
+// of 2^8 that keeps small f16 weights normal.  f32: m16n8k8 on tf32 halves of
+// each operand (11 + 11 bits; high x high + high x low + low x high), within
+// 2^-21 of each product.
+template <typename T>
+struct Tile;
+template <>
+struct Tile<float> {
+  static constexpr int kKeys = 32;
+};
+template <>
+struct Tile<__half> {
+  static constexpr int kKeys = 64;
+};
+template <>
+struct Tile<__nv_bfloat16> {
+  static constexpr int kKeys = 64;
+};
+
+constexpr int kStages = 2;
+constexpr float kShift = 8.0f;
+
+template <typename T, int D>
+constexpr int pitch() {
+  return D + 8;
+}
+template <typename T, int D>
+constexpr int stage_elems() {
+  return Tile<T>::kKeys * pitch<T, D>();  // one of K and V
+}
+template <typename T, int D>
+constexpr int cross_smem() {
+  return kStages * (2 * stage_elems<T, D>() * (int)sizeof(T) + 16);
+}
+
+__device__ __forceinline__ void cp16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = high + low: the upper 11 bits of the mantissa, and the rest.
+__device__ __forceinline__ uint32_t tf32_high(float x) { return __float_as_uint(x) & 0xFFFFE000u; }
+__device__ __forceinline__ uint32_t tf32_low(float x) {
+  return __float_as_uint(__fsub_rn(x, __uint_as_float(__float_as_uint(x) & 0xFFFFE000u)));
+}
+__device__ __forceinline__ void mma_split(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0,
+                                          float b1) {
+  const uint32_t h0 = tf32_high(b0), h1 = tf32_high(b1);
+  mma_tf32(d, al, h0, h1);
+  mma_tf32(d, ah, tf32_low(b0), tf32_low(b1));
+  mma_tf32(d, ah, h0, h1);
+}
+
+template <typename T, int D, int WR>
+__global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int kKeys = Tile<T>::kKeys, kGroups = 4 / WR, kOwn = kKeys / kGroups, kNT = kOwn / 8;
+  constexpr int kPitch = pitch<T, D>(), kElems = stage_elems<T, D>(), kRows = 16 * WR;
+  constexpr int kChunk = 16 / (int)sizeof(T), kRowChunks = D / kChunk;
+  constexpr int kOut = D / 8;  // n8 tiles of the output
+  extern __shared__ __align__(128) uint8_t smem[];
+  T* ring = reinterpret_cast<T*>(smem);
+  uint32_t* live_bits = reinterpret_cast<uint32_t*>(smem + kStages * 2 * kElems * sizeof(T));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int wr = warp % WR, kg = warp / WR;
+  pdl_enter();
+
+  const AttnRows& r = p.rows;
+  const long long unit = blockIdx.x, bh = unit / p.row_tiles;
+  const int tile = (int)(unit - bh * p.row_tiles), b = (int)(bh / r.kv_heads), head = (int)(bh - (long long)b * r.kv_heads);
+  const int split = blockIdx.y;
+  const AttnSeq seq = attn_seq(r, b, p.status, head == 0 && tile == 0 && split == 0 && tid == 0);
+  const int n_rows = seq.nq * r.group, row0 = tile * kRows;
+  if (!seq.ok || row0 >= n_rows) return;
+  const int n_tiles = (seq.nk + kKeys - 1) / kKeys;
+  const int parts = max(1, (n_tiles + p.split.chunk - 1) / p.split.chunk);
+  if (split >= parts) return;
+  const int begin = split * p.split.chunk, end = min(n_tiles, begin + p.split.chunk);
+
+  const T* kbase = static_cast<const T*>(p.k) + (long long)seq.k0 * p.k_rs + (long long)head * p.k_hs;
+  const T* vbase = static_cast<const T*>(p.v) + (long long)seq.k0 * p.v_rs + (long long)head * p.v_hs;
+  const uint8_t* mask = p.mask ? p.mask + seq.k0 : nullptr;
+
+  auto load_tile = [&](int tl) {
+    const int s = tl & (kStages - 1), key0 = tl * kKeys;
+    T* ks = ring + s * 2 * kElems;
+    T* vs = ks + kElems;
+    if (warp < kKeys / 32) {
+      const int key = key0 + warp * 32 + lane;
+      const uint32_t w = __ballot_sync(kFull, key < seq.nk && (!mask || mask[key]));
+      if (lane == 0) live_bits[s * 2 + warp] = w;
+    }
+#pragma unroll
+    for (int c = tid; c < kKeys * kRowChunks; c += 128) {
+      const int row = c / kRowChunks, at = (c - row * kRowChunks) * kChunk;
+      const int key = key0 + row;
+      // A key that is left out is zeros, whatever it holds: a weight of 0
+      // times an infinity would be NaN.
+      const bool there = key < seq.nk && (!mask || mask[key]);
+      const int from = there ? key : 0;
+      cp16(ks + row * kPitch + at, kbase + (long long)from * p.k_rs + at, there);
+      cp16(vs + row * kPitch + at, vbase + (long long)from * p.v_rs + at, there);
+    }
+    cp_commit();
+  };
+  if (begin < end) load_tile(begin);
+
+  // ---- the warp's 16 query rows ----
+  const int own = row0 + wr * 16;
+  const void* src[2];
+  bool there[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = own + g + 8 * h;
+    there[h] = row < n_rows;
+    const int pos = there[h] ? row / r.group : 0, qh = head * r.group + (there[h] ? row - pos * r.group : 0);
+    src[h] = static_cast<const T*>(r.q) + (long long)(seq.q0 + pos) * r.q_row_stride + (long long)qh * r.q_head_stride;
+  }
+  const bool busy = own < n_rows;
+  uint32_t qa[kF32 ? D / 8 : D / 16][4];
+  if (kF32) {
+    // step s: k = t is channel 8 s + 2 t, k = t + 4 the one after it
+#pragma unroll
+    for (int s = 0; s < D / 8; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float2 v = there[h] ? *reinterpret_cast<const float2*>(static_cast<const float*>(src[h]) + 8 * s + 2 * t)
+                                  : make_float2(0.0f, 0.0f);
+        qa[s][h] = __float_as_uint(v.x);
+        qa[s][2 + h] = __float_as_uint(v.y);
+      }
+  } else {
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          qa[s % (kF32 ? D / 8 : D / 16)][2 * e + h] =
+              there[h] ? *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(src[h]) + 16 * s + 8 * e + 2 * t)
+                       : 0u;
+  }
+
+  const float factor = __fmul_rn(p.scale, kLog2e);
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+  float acc[kOut][4];
+#pragma unroll
+  for (int i = 0; i < kOut; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+
+  for (int tl = begin; tl < end; ++tl) {
+    if (tl + 1 < end) {
+      load_tile(tl + 1);
+      cp_wait<1>();
+    } else {
+      cp_wait<0>();
+    }
+    __syncthreads();
+    if (busy) {
+      const int s = tl & (kStages - 1);
+      const T* ks = ring + s * 2 * kElems + kg * kOwn * kPitch;
+      const T* vs = ks + kElems;
+      float x[kNT][4];
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j][e] = 0.0f;
+      // column n of a score tile: key n (16 bits), or key (n / 2) + 4 (n % 2)
+      // (f32), so that a thread's two columns are the rows t and t + 4 of the
+      // values, which lie in different banks
+      if constexpr (kF32) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint32_t ah[4], al[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            ah[e] = tf32_high(__uint_as_float(qa[c][e]));
+            al[e] = tf32_low(__uint_as_float(qa[c][e]));
+          }
+#pragma unroll
+          for (int j = 0; j < kNT; ++j) {
+            const float2 kv = *reinterpret_cast<const float2*>(ks + (8 * j + (g >> 1) + 4 * (g & 1)) * kPitch + 8 * c + 2 * t);
+            mma_split(x[j], ah, al, kv.x, kv.y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+          for (int j = 0; j < kNT; j += 2) {
+            uint32_t kb[4];
+            ldsm4(kb, ks + (8 * j + (lane & 7) + (lane >> 4) * 8) * kPitch + 16 * c + ((lane >> 3) & 1) * 8);
+            if constexpr (sizeof(T) == 2) {
+              if (std::is_same<T, __half>::value) {
+                mma_f16(x[j], qa[c][0], qa[c][1], qa[c][2], qa[c][3], kb[0], kb[1]);
+                mma_f16(x[j + 1], qa[c][0], qa[c][1], qa[c][2], qa[c][3], kb[2], kb[3]);
+              } else {
+                mma_bf16(x[j], qa[c][0], qa[c][1], qa[c][2], qa[c][3], kb[0], kb[1]);
+                mma_bf16(x[j + 1], qa[c][0], qa[c][1], qa[c][2], qa[c][3], kb[2], kb[3]);
+              }
+            }
+          }
+      }
+      // ---- scale, mask, running maximum ----
+      uint32_t bits[(kOwn + 31) / 32];
+      bool all = true;
+#pragma unroll
+      for (int w = 0; w < (kOwn + 31) / 32; ++w) {
+        const int at = kg * kOwn + 32 * w;
+        bits[w] = live_bits[s * 2 + (at >> 5)] >> (at & 31);
+        const uint32_t want = kOwn >= 32 ? kFull : (1u << (kOwn & 31)) - 1u;
+        all = all && (bits[w] & want) == want;
+      }
+      float most[2] = {top[0], top[1]};
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[j][e] = __fmul_rn(x[j][e], factor);
+          const int key = 8 * j + (kF32 ? t + 4 * (e & 1) : 2 * t + (e & 1));
+          if (!all && !(bits[key >> 5] >> (key & 31) & 1)) x[j][e] = -INFINITY;
+          most[e >> 1] = fmaxf(most[e >> 1], x[j][e]);
+        }
+      float base[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        most[h] = fmaxf(most[h], __shfl_xor_sync(kFull, most[h], 1));
+        most[h] = fmaxf(most[h], __shfl_xor_sync(kFull, most[h], 2));
+      }
+      if (__any_sync(kFull, most[0] > top[0] || most[1] > top[1])) {
+        float shrink[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          shrink[h] = top[h] == -INFINITY ? 0.0f : exp2_approx(__fsub_rn(top[h], most[h]));
+          top[h] = most[h];
+          sum[h] = __fmul_rn(sum[h], shrink[h]);
+        }
+#pragma unroll
+        for (int i = 0; i < kOut; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][e] = __fmul_rn(acc[i][e], shrink[e >> 1]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) base[h] = top[h] == -INFINITY ? 0.0f : __fsub_rn(top[h], kShift);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[j][e] = exp2_approx(__fsub_rn(x[j][e], base[e >> 1]));
+          sum[e >> 1] = __fadd_rn(sum[e >> 1], x[j][e]);
+        }
+      // ---- values ----
+      if constexpr (kF32) {
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+          uint32_t ah[4], al[4];
+          // k = t: column 2 t (key t); k = t + 4: column 2 t + 1 (key t + 4)
+          ah[0] = tf32_high(x[j][0]); ah[1] = tf32_high(x[j][2]); ah[2] = tf32_high(x[j][1]); ah[3] = tf32_high(x[j][3]);
+          al[0] = tf32_low(x[j][0]); al[1] = tf32_low(x[j][2]); al[2] = tf32_low(x[j][1]); al[3] = tf32_low(x[j][3]);
+          const T* v0 = vs + (8 * j + t) * kPitch + 2 * g;
+          const T* v1 = v0 + 4 * kPitch;
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            const float2 a = *reinterpret_cast<const float2*>(v0 + 16 * c), e = *reinterpret_cast<const float2*>(v1 + 16 * c);
+            mma_split(acc[2 * c], ah, al, a.x, e.x);
+            mma_split(acc[2 * c + 1], ah, al, a.y, e.y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kNT; j += 2) {
+          uint32_t a[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float lo = x[j + (e >> 1)][2 * (e & 1)], hi = x[j + (e >> 1)][2 * (e & 1) + 1];
+            a[e] = std::is_same<T, __half>::value ? pack_f16(lo, hi) : pack_bf16(lo, hi);
+          }
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t vb[4];
+            ldsm4t(vb, vs + (8 * j + (lane & 15)) * kPitch + 16 * c + (lane >> 4) * 8);
+            if (std::is_same<T, __half>::value) {
+              mma_f16(acc[2 * c], a[0], a[1], a[2], a[3], vb[0], vb[1]);
+              mma_f16(acc[2 * c + 1], a[0], a[1], a[2], a[3], vb[2], vb[3]);
+            } else {
+              mma_bf16(acc[2 * c], a[0], a[1], a[2], a[3], vb[0], vb[1]);
+              mma_bf16(acc[2 * c + 1], a[0], a[1], a[2], a[3], vb[2], vb[3]);
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // ---- normalize ----
+  float inv[2], lse2[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    sum[h] = __fadd_rn(sum[h], __shfl_xor_sync(kFull, sum[h], 1));
+    sum[h] = __fadd_rn(sum[h], __shfl_xor_sync(kFull, sum[h], 2));
+    inv[h] = sum[h] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum[h]);
+    lse2[h] = sum[h] == 0.0f ? -INFINITY : __fadd_rn(__fsub_rn(top[h], kShift), log2f(sum[h]));
+  }
+  const long long slot0 = unit * kRows;
+  const bool direct = parts <= 1;
+  auto emit = [&](int row, int ch, float a, float e) {  // row of the unit
+    if (direct) {
+      const int pos = (row0 + row) / r.group, h = head * r.group + (row0 + row) - pos * r.group;
+      store2(r.out, (long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride + ch, r.dtype, a, e);
+    } else {
+      *reinterpret_cast<float2*>(p.split.out + ((slot0 + row) * p.split.splits + split) * D + ch) = make_float2(a, e);
+    }
+  };
+  auto emit_lse = [&](int row, float l) {
+    if (!direct) {
+      p.split.lse[(slot0 + row) * p.split.splits + split] = l;
+    } else if (r.lse) {
+      const int pos = (row0 + row) / r.group, h = head * r.group + (row0 + row) - pos * r.group;
+      r.lse[(long long)(seq.q0 + pos) * r.kv_heads * r.group + h] = __fmul_rn(l, kLn2);
+    }
+  };
+  float* part = reinterpret_cast<float*>(smem) + (kg * WR + wr) * 16 * (D + 1);
+#pragma unroll
+  for (int i = 0; i < kOut; i += (kF32 ? 2 : 1))
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = wr * 16 + g + 8 * h;
+      if (row0 + row >= n_rows) continue;
+      if constexpr (kF32) {
+        // tiles i, i + 1: channels 8 i + 4 t + {0, 1} of column 2 t, + {2, 3} of column 2 t + 1
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float a = __fmul_rn(acc[i][2 * h + e], inv[h]), c = __fmul_rn(acc[i + 1][2 * h + e], inv[h]);
+          const int ch = 8 * i + 4 * t + 2 * e;
+          if (kGroups == 1) {
+            emit(row, ch, a, c);
+          } else {
+            part[(g + 8 * h) * D + ch] = a;
+            part[(g + 8 * h) * D + ch + 1] = c;
+          }
+        }
+      } else {
+        const float a = __fmul_rn(acc[i][2 * h], inv[h]), c = __fmul_rn(acc[i][2 * h + 1], inv[h]);
+        const int ch = 8 * i + 2 * t;
+        if (kGroups == 1) {
+          emit(row, ch, a, c);
+        } else {
+          part[(g + 8 * h) * D + ch] = a;
+          part[(g + 8 * h) * D + ch + 1] = c;
+        }
+      }
+    }
+  if (t == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = wr * 16 + g + 8 * h;
+      if (row0 + row >= n_rows) continue;
+      if (kGroups == 1)
+        emit_lse(row, lse2[h]);
+      else
+        part[16 * D + g + 8 * h] = lse2[h];
+    }
+  }
+  if (kGroups == 1) return;
+  __syncthreads();
+  // ---- join the key groups: warp w takes every fourth row ----
+  for (int row = warp; row < kRows && row0 + row < n_rows; row += 4) {
+    const float* of = reinterpret_cast<const float*>(smem) + (row / 16) * 16 * (D + 1);
+    constexpr int kStep = WR * 16 * (D + 1);
+    float w[kGroups], best = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      w[k] = of[k * kStep + 16 * D + row % 16];
+      best = fmaxf(best, w[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      w[k] = w[k] != w[k] ? w[k] : join_weight(w[k], best);
+      total = __fadd_rn(total, w[k]);
+    }
+    const float scale = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+    for (int ch = 2 * lane; ch < D; ch += 64) {
+      float a = 0.0f, e = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k)
+        if (w[k] != 0.0f) {
+          a = __fmaf_rn(w[k], of[k * kStep + (row % 16) * D + ch], a);
+          e = __fmaf_rn(w[k], of[k * kStep + (row % 16) * D + ch + 1], e);
+        }
+      emit(row, ch, __fmul_rn(a, scale), __fmul_rn(e, scale));
+    }
+    if (lane == 0) emit_lse(row, total == 0.0f ? -INFINITY : __fadd_rn(best, log2f(total)));
+  }
+}
+
+// ---- shapes of a launch ----
+struct CrossPlan {
+  int warps_rows, row_tiles, splits, chunk, tile_keys;
+  long long units;
+  uint64_t slots, bytes;
+};
+
+bool cross_plan(const mc_cross_attention_args* a, CrossPlan* plan) {
+  if (!a || dtype_bytes(a->dtype) == 0 || a->batch < 0 || a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads != 0 ||
+      a->head_dim < 16 || a->head_dim > kOpMaxHeadDim || a->head_dim % 16 != 0 || a->max_q_len < 0 || a->max_k_len < 0 ||
+      a->heads > 65536)
+    return false;
+  const int64_t rows = (int64_t)(a->heads / a->kv_heads) * a->max_q_len;
+  if (rows > INT32_MAX / 2) return false;
+  plan->tile_keys = a->dtype == MC_F32 ? 32 : 64;
+  plan->warps_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int tile_rows = 16 * plan->warps_rows;
+  plan->row_tiles = (int)((rows + tile_rows - 1) / tile_rows);
+  plan->units = (int64_t)a->batch * a->kv_heads * plan->row_tiles;
+  if (plan->units > INT32_MAX) return false;
+  // Ranges of keys for units too few to fill the GPU (three CTAs per SM),
+  // each of four tiles at least.
+  const int tiles = (int)(((int64_t)a->max_k_len + plan->tile_keys - 1) / plan->tile_keys);
+  long long splits = plan->units > 0 ? kSms * 3 / plan->units : 1;
+  if (splits > tiles / 4) splits = tiles / 4;
+  if (splits > 256) splits = 256;
+  if (splits < 1) splits = 1;
+  plan->chunk = tiles > 0 ? (int)((tiles + splits - 1) / splits) : 1;
+  plan->splits = tiles > 0 ? (tiles + plan->chunk - 1) / plan->chunk : 1;
+  plan->slots = (uint64_t)plan->units * tile_rows;
+  plan->bytes = attn_split_bytes(plan->slots, plan->splits, a->head_dim);
+  return true;
+}
+
+template <typename T, int D, int WR>
+cudaError_t launch_small(const CrossParams& p, const CrossPlan& plan, cudaStream_t s) {
+  static uint64_t done = 0;
+  constexpr int bytes = cross_smem<T, D>();
+  cudaError_t e = allow_smem(cross_small_kernel<T, D, WR>, bytes, &done);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(cross_small_kernel<T, D, WR>, dim3((unsigned)plan.units, plan.splits), dim3(128), bytes, s, p);
+}
+
+template <typename T, int D>
+cudaError_t launch_small_w(const CrossParams& p, const CrossPlan& plan, cudaStream_t s) {
+  return plan.warps_rows == 1   ? launch_small<T, D, 1>(p, plan, s)
+         : plan.warps_rows == 2 ? launch_small<T, D, 2>(p, plan, s)
+                                : launch_small<T, D, 4>(p, plan, s);
+}
+
+template <int D>
+cudaError_t launch_small_t(const CrossParams& p, const CrossPlan& plan, cudaStream_t s) {
+  return p.rows.dtype == MC_F32   ? launch_small_w<float, D>(p, plan, s)
+         : p.rows.dtype == MC_F16 ? launch_small_w<__half, D>(p, plan, s)
+                                  : launch_small_w<__nv_bfloat16, D>(p, plan, s);
+}
+
+}  // namespace
+}  // namespace mc
+
+extern "C" uint64_t mc_cross_attention_workspace(const mc_cross_attention_args* args) {
+  mc::CrossPlan plan;
+  return mc::cross_plan(args, &plan) ? plan.bytes : 0;
+}
+
+extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* stream) {
+  mc::CrossPlan plan;
+  if (!mc::cross_plan(a, &plan) || !isfinite(a->scale) || a->q_rows < 0 || a->q_rows > INT32_MAX || a->k_rows < 0 ||
+      a->k_rows > INT32_MAX)
+    return MC_INVALID_INPUT;
+  if (plan.units == 0) return MC_OK;
+  const int bytes = mc::dtype_bytes(a->dtype);
+  if (!a->q_start || !a->q_len || !a->k_start || !a->k_len || !mc::aligned4(a->q_start) || !mc::aligned4(a->q_len) ||
+      !mc::aligned4(a->k_start) || !mc::aligned4(a->k_len) || !mc::aligned4(a->lse) ||
+      !mc::strides_ok(a->q, a->q_row_stride, a->q_head_stride, bytes) ||
+      !mc::strides_ok(a->k, a->k_row_stride, a->k_head_stride, bytes) ||
+      !mc::strides_ok(a->v, a->v_row_stride, a->v_head_stride, bytes) ||
+      !mc::strides_ok(a->out, a->out_row_stride, a->out_head_stride, bytes) ||
+      !mc::strides_apart(a->q_rows, a->heads, a->head_dim, a->out_row_stride, a->out_head_stride) || a->out == a->q ||
+      a->out == a->k || a->out == a->v)
+    return MC_INVALID_INPUT;
+  if (plan.bytes > 0 && (!a->workspace || !mc::aligned16(a->workspace) || a->workspace_bytes < plan.bytes))
+    return MC_INVALID_INPUT;
+  mc_status where = mc::on_current_device(a->q);
+  if (where == MC_OK) where = mc::on_current_device(a->k);
+  if (where != MC_OK) return where;
+  uint32_t* status = mc::op_status_word();
+  if (!status) return MC_CUDA;
+  mc::CrossParams p;
+  std::memset(&p, 0, sizeof(p));
+  mc::AttnRows& r = p.rows;
+  r.q = a->q;
+  r.out = a->out;
+  r.lse = a->lse;
+  r.q_start = a->q_start;
+  r.q_len = a->q_len;
+  r.k_len = a->k_len;
+  r.k_start = a->k_start;
+  r.q_rows = a->q_rows;
+  r.k_rows = a->k_rows;
+  r.q_row_stride = a->q_row_stride;
+  r.q_head_stride = a->q_head_stride;
+  r.out_row_stride = a->out_row_stride;
+  r.out_head_stride = a->out_head_stride;
+  r.dtype = a->dtype;
+  r.batch = a->batch;
+  r.kv_heads = a->kv_heads;
+  r.group = a->heads / a->kv_heads;
+  r.head_dim = a->head_dim;
+  r.max_q = a->max_q_len;
+  r.max_k = a->max_k_len;
+  p.split.splits = plan.splits;
+  p.split.chunk = plan.chunk;
+  if (plan.splits > 1) {
+    p.split.out = static_cast<float*>(a->workspace);
+    p.split.lse = p.split.out + plan.slots * plan.splits * a->head_dim;
+  }
+  p.k = a->k;
+  p.v = a->v;
+  p.k_rs = a->k_row_stride;
+  p.k_hs = a->k_head_stride;
+  p.v_rs = a->v_row_stride;
+  p.v_hs = a->v_head_stride;
+  p.mask = a->key_mask;
+  p.scale = a->scale;
+  p.row_tiles = plan.row_tiles;
+  p.status = status;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaErrorInvalidValue;
+  switch (a->head_dim) {
+    case 16: e = mc::launch_small_t<16>(p, plan, s); break;
+    case 32: e = mc::launch_small_t<32>(p, plan, s); break;
+    case 48: e = mc::launch_small_t<48>(p, plan, s); break;
+    case 64: e = mc::launch_small_t<64>(p, plan, s); break;
+    case 80: e = mc::launch_small_t<80>(p, plan, s); break;
+    case 96: e = mc::launch_small_t<96>(p, plan, s); break;
+    case 112: e = mc::launch_small_t<112>(p, plan, s); break;
+    case 128: e = mc::launch_small_t<128>(p, plan, s); break;
+  }
+  if (e != cudaSuccess) return MC_CUDA;
+  if (plan.splits > 1)
+    e = mc::launch_attn_join(r, p.split, plan.tile_keys, 16 * plan.warps_rows, plan.row_tiles, s);
+  return e == cudaSuccess ? MC_OK : MC_CUDA;
+}

@@ -22,7 +22,7 @@ EXPORTS = [
     "mc_segment_text", "mc_timeline", "mc_timeline_read", "mc_inspect_marian_bin",
     "mc_encode_token_ids", "mc_replay",
     "mc_kv4_page_bytes", "mc_kv4_append", "mc_kv4_read", "mc_kv4_attention_workspace", "mc_kv4_attention",
-    "mc_sample",
+    "mc_cross_attention_workspace", "mc_cross_attention", "mc_sample",
 ]
 
 # MC_Q8_LINEAR_NOALLOC_MAX_ACTIVATIONS in include/marian_cuda.h
@@ -93,6 +93,18 @@ class Kv4AttentionArgs(C.Structure):
                 ("q_head_stride", C.c_int64), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64),
                 ("dtype", C.c_int32), ("heads", C.c_int32), ("max_q_len", C.c_int32), ("max_kv_len", C.c_int32),
                 ("causal", C.c_int32), ("scale", C.c_float)]
+
+
+class CrossAttentionArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("q_start", C.c_void_p), ("q_len", C.c_void_p), ("k_start", C.c_void_p), ("k_len", C.c_void_p),
+                ("key_mask", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                ("q_rows", C.c_int64), ("k_rows", C.c_int64), ("q_row_stride", C.c_int64),
+                ("q_head_stride", C.c_int64), ("k_row_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_row_stride", C.c_int64), ("v_head_stride", C.c_int64), ("out_row_stride", C.c_int64),
+                ("out_head_stride", C.c_int64), ("dtype", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("max_q_len", C.c_int32),
+                ("max_k_len", C.c_int32), ("scale", C.c_float)]
 
 
 class SampleArgs(C.Structure):
@@ -168,6 +180,9 @@ def load(build_if_missing: bool = True):
     lib.mc_kv4_attention_workspace.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionArgs)]
     lib.mc_kv4_attention_workspace.restype = u64
     lib.mc_kv4_attention.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionArgs), vp]
+    lib.mc_cross_attention_workspace.argtypes = [C.POINTER(CrossAttentionArgs)]
+    lib.mc_cross_attention_workspace.restype = u64
+    lib.mc_cross_attention.argtypes = [C.POINTER(CrossAttentionArgs), vp]
     lib.mc_sample.argtypes = [C.POINTER(SampleArgs), vp]
     lib.mc_launch_count.argtypes = [vp]
     lib.mc_launch_count.restype = u64

@@ -1,0 +1,372 @@
+"""mc_cross_attention against a plain 64-bit form: packed and padded batches,
+single tokens, shared heads and keys, masks, odd head sizes and lengths, split
+keys, strides, infinities and NaN where the mask leaves keys out.
+
+Tolerances, derived from the arithmetic.  f32: a product of three tf32 halves
+is within 2^-21 of its value and a score's f32 sum loses at most 2^-21 more of
+sum|q||k|: dx = 2^-20 * scale * sum|q| max|k|, which moves an output by at most
+2 dx max|v|; the weighted sum and the sum of weights lose 2^-19 of max|v| each.
+16 bits: products are exact; weights and output are rounded to the type, half
+a step each: (eps / 2 + eps / 2 + 2 dx) max|v|.  The f32 errors are
+independent, so their root mean square stays below 2^-19 max|v|.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from marian_cuda import _lib as L  # noqa: E402
+
+gpu = pytest.mark.gpu
+DTYPES = {"f32": (torch.float32, L.MC_F32), "f16": (torch.float16, L.MC_F16), "bf16": (torch.bfloat16, L.MC_BF16)}
+
+
+def attend(q, k, v, scale, live):
+    """q [m, h, d], k, v [n, hk, d] float64, live [n] -> out [m, h, d], lse [m, h]."""
+    m, h, d = q.shape
+    k, v = k[live], v[live]
+    out, lse = np.zeros((m, h, d)), np.full((m, h), -np.inf)
+    if k.shape[0] == 0:
+        return out, lse
+    for j in range(h):
+        x = q[:, j] @ k[:, j * k.shape[1] // h].T * scale
+        top = x.max(1, keepdims=True)
+        w = np.exp(x - top)
+        out[:, j] = w @ v[:, j * k.shape[1] // h] / w.sum(1, keepdims=True)
+        lse[:, j] = top[:, 0] + np.log(w.sum(1))
+    return out, lse
+
+
+def ints(a):
+    return torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()
+
+
+def typed(rng, shape, dtype, size=1.0):
+    return torch.from_numpy((rng.standard_normal(shape) * size).astype(np.float32)).to(DTYPES[dtype][0])
+
+
+def f64(x):
+    return x.float().cpu().numpy().astype(np.float64)
+
+
+def status_bits():
+    bits = C.c_uint32(0)
+    assert L.load().mc_op_status(C.byref(bits)) == L.MC_OK
+    return bits.value
+
+
+def arguments(q, k, v, out, lse, lens, mask, dtype, scale, max_q, max_k):
+    a = L.CrossAttentionArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), lse=None if lse is None else lse.data_ptr(),
+        q_start=lens[0].data_ptr(), q_len=lens[1].data_ptr(), k_start=lens[2].data_ptr(), k_len=lens[3].data_ptr(),
+        key_mask=None if mask is None else mask.data_ptr(), q_rows=q.shape[0], k_rows=k.shape[0],
+        q_row_stride=q.stride(0), q_head_stride=q.stride(1), k_row_stride=k.stride(0), k_head_stride=k.stride(1),
+        v_row_stride=v.stride(0), v_head_stride=v.stride(1), out_row_stride=out.stride(0),
+        out_head_stride=out.stride(1), dtype=DTYPES[dtype][1], batch=lens[0].shape[0], heads=q.shape[1],
+        kv_heads=k.shape[1], head_dim=q.shape[2], max_q_len=max_q, max_k_len=max_k, scale=scale)
+    need = L.load().mc_cross_attention_workspace(C.byref(a))
+    ws = torch.empty(max(1, need), dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    a.keep = (ws, lens, mask, q, k, v, out, lse)
+    return a, need
+
+
+def run(q, k, v, q_start, q_len, k_start, k_len, dtype, scale, mask=None, max_q=None, max_k=None, out=None):
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda") if out is None else out
+    lse = torch.full(q.shape[:2], 7.0, device="cuda")
+    lens = [ints(x) for x in (q_start, q_len, k_start, k_len)]
+    m = None if mask is None else torch.from_numpy(np.asarray(mask, np.uint8)).cuda()
+    a, need = arguments(q, k, v, out, lse, lens, m, dtype, scale, int(max(q_len)) if max_q is None else max_q,
+                        int(max(k_len)) if max_k is None else max_k)
+    torch.cuda.synchronize()
+    assert L.load().mc_cross_attention(C.byref(a), torch.cuda.current_stream().cuda_stream) == L.MC_OK
+    torch.cuda.synchronize()
+    return out, lse, need
+
+
+def compare(q, k, v, out, lse, q_start, q_len, k_start, k_len, dtype, scale, mask=None):
+    qd, kd, vd, od, ld = (f64(x) for x in (q, k, v, out, lse))
+    eps = torch.finfo(q.dtype).eps
+    touched = np.zeros(q.shape[0], bool)
+    for q0, m, k0, n in zip(q_start, q_len, k_start, k_len):
+        at = slice(q0, q0 + m)
+        touched[at] = True
+        if m == 0:
+            continue
+        live = np.ones(n, bool) if mask is None else np.asarray(mask[k0:k0 + n]) != 0
+        want, wl = attend(qd[at], kd[k0:k0 + n], vd[k0:k0 + n], scale, live)
+        some = live.any()
+        big = np.abs(vd[k0:k0 + n][live]).max() if some else 1.0
+        dx = 2.0 ** -20 * scale * np.abs(qd[at]).sum(-1).max() * np.abs(kd[k0:k0 + n][live]).max() if some else 0.0
+        tol = (2.0 ** -18 if dtype == "f32" else eps) + 2 * dx
+        np.testing.assert_allclose(od[at], want, rtol=0, atol=tol * big)
+        if dtype == "f32":
+            assert np.sqrt(np.mean((od[at] - want) ** 2)) <= 2.0 ** -19 * big
+        np.testing.assert_allclose(ld[at], wl, rtol=2.0 ** -20, atol=2.0 ** -19 + dx)
+    assert (od[~touched] == 7).all() and (ld[~touched] == 7).all()
+
+
+def check(rng, q_len, k_len, h, hk, d, dtype, mask=None, gap_q=0, gap_k=0, size=1.0):
+    b = len(q_len)
+    q_start = np.cumsum(q_len) - q_len + gap_q * np.arange(b)
+    k_start = np.cumsum(k_len) - k_len + gap_k * np.arange(b)
+    rows_q, rows_k = int(np.sum(q_len)) + gap_q * b + 1, int(np.sum(k_len)) + gap_k * b + 1
+    q, k, v = typed(rng, (rows_q, h, d), dtype, size), typed(rng, (rows_k, hk, d), dtype), typed(rng, (rows_k, hk, d), dtype)
+    m = None
+    if mask is not None:
+        m = (rng.random(rows_k) < mask).astype(np.uint8)
+        m[k_start[0]:k_start[0] + k_len[0]] = 0     # nothing left of the first
+    # what no query may see is not finite
+    seen = np.zeros(rows_k, bool)
+    for k0, n in zip(k_start, k_len):
+        seen[k0:k0 + n] = True if m is None else m[k0:k0 + n] != 0
+    lost = torch.from_numpy(~seen)
+    k[lost], v[lost] = float("nan"), float("inf")
+    scale = d ** -0.5
+    out, lse, need = run(q.cuda(), k.cuda(), v.cuda(), q_start, q_len, k_start, k_len, dtype, scale, m)
+    assert status_bits() == 0
+    compare(q, k, v, out, lse, q_start, q_len, k_start, k_len, dtype, scale, m)
+    return need
+
+
+# ---- refusals ------------------------------------------------------------------
+
+def host_args():
+    return L.CrossAttentionArgs(q=1 << 20, k=2 << 20, v=3 << 20, out=4 << 20, lse=64, q_start=64, q_len=64, k_start=64,
+                                k_len=64, workspace=1 << 20, workspace_bytes=1 << 40, q_rows=10, k_rows=20,
+                                q_row_stride=256, q_head_stride=64, k_row_stride=128, k_head_stride=64,
+                                v_row_stride=128, v_head_stride=64, out_row_stride=256, out_head_stride=64,
+                                dtype=L.MC_F32, batch=2, heads=4, kv_heads=2, head_dim=64, max_q_len=5, max_k_len=10,
+                                scale=0.125)
+
+
+@pytest.mark.parametrize("field,value", [
+    ("q", 0), ("k", 0), ("v", 0), ("out", 0), ("q", (1 << 20) + 8), ("k", (2 << 20) + 4), ("out", 1 << 20),
+    ("out", 2 << 20), ("out", 3 << 20), ("lse", 2), ("q_start", 0), ("q_len", 0), ("k_start", 0), ("k_len", 0),
+    ("k_len", 66), ("q_rows", -1), ("k_rows", -1), ("k_rows", 1 << 31), ("q_row_stride", 254), ("k_row_stride", -128),
+    ("v_head_stride", 62), ("out_head_stride", 32), ("out_row_stride", 64), ("out_row_stride", 0), ("dtype", 3),
+    ("dtype", -1), ("batch", -1), ("heads", 3), ("heads", 0), ("kv_heads", 0), ("kv_heads", -2), ("head_dim", 24),
+    ("head_dim", 0), ("head_dim", 144), ("max_q_len", -1), ("max_k_len", -1), ("scale", float("nan")),
+    ("scale", float("-inf"))])
+def test_bad_arguments_are_refused(field, value):
+    a = host_args()
+    setattr(a, field, value)
+    assert L.load().mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
+
+
+def test_strides_of_16_bit_rows_are_checked_in_bytes():
+    a = host_args()
+    a.dtype, a.k_row_stride = L.MC_BF16, 132   # 264 bytes
+    assert L.load().mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
+
+
+def test_null_empty_and_short_workspace():
+    lib = L.load()
+    assert lib.mc_cross_attention(None, None) == L.MC_INVALID_INPUT
+    assert lib.mc_cross_attention_workspace(None) == 0
+    for field in ("batch", "max_q_len"):
+        a = host_args()
+        setattr(a, field, 0)
+        assert lib.mc_cross_attention(C.byref(a), None) == L.MC_OK
+    a = host_args()
+    a.batch, a.max_q_len, a.max_k_len = 1, 1, 20000
+    need = lib.mc_cross_attention_workspace(C.byref(a))
+    assert need > 0
+    for ws, n in ((0, need), (1 << 20, need - 1), ((1 << 20) + 4, need)):
+        a.workspace, a.workspace_bytes = ws, n
+        assert lib.mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
+    if not torch.cuda.is_available():
+        assert lib.mc_cross_attention(C.byref(host_args()), None) == L.MC_CUDA
+
+
+@gpu
+def test_host_memory_is_refused():
+    a = host_args()
+    host = torch.zeros(4096)
+    a.q = (host.data_ptr() + 15) // 16 * 16
+    assert L.load().mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
+
+
+# ---- the definition --------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128])
+def test_single_tokens(dtype, d):
+    rng = np.random.default_rng(d)
+    k_len = [1, 0, 7, 31, 32, 33, 63, 64, 65, 127, 256]
+    check(rng, [1] * len(k_len), k_len, 2, 2, d, dtype, gap_k=1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,hk,group", [(64, 2, 1), (48, 1, 8), (128, 2, 4), (80, 3, 7), (16, 1, 3)])
+@pytest.mark.parametrize("top", [3, 30, 200])
+def test_ragged_batches_with_shared_heads(dtype, d, hk, group, top):
+    rng = np.random.default_rng(d + top)
+    q_len = [top, 1, 0, 2, max(1, top // 2 + 1)]
+    k_len = [3, 200, 40, 0, 65]
+    check(rng, q_len, k_len, hk * group, hk, d, dtype, gap_q=2, gap_k=3)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,q_len", [(64, 1), (48, 20), (128, 70), (96, 33)])
+def test_padded_batches_with_masks(dtype, d, q_len):
+    rng = np.random.default_rng(q_len)
+    check(rng, [q_len, q_len, q_len, q_len - 1], [100, 130, 64, 1], 4, 2, d, dtype, mask=0.6, gap_q=4, gap_k=30)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_len,k_len,h,hk", [([1], [1000], 1, 1), ([1, 1], [2500, 3], 8, 2), ([5], [4097], 2, 2),
+                                             ([40, 40], [3000, 0], 2, 1), ([1], [300], 8, 8)])
+def test_split_keys(dtype, q_len, k_len, h, hk):
+    rng = np.random.default_rng(k_len[0])
+    for mask in (None, 0.5):
+        if mask is None or len(q_len) > 1:
+            check(rng, q_len, k_len, h, hk, 64, dtype, mask=mask)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d,q_len,k_len,h,hk", [(128, [300, 129], [1000, 257], 4, 2), (64, [513], [640], 2, 2),
+                                               (48, [128, 128], [129, 4095], 2, 1), (112, [255], [128], 2, 2),
+                                               (96, [700], [1], 1, 1), (16, [256], [333], 2, 2), (32, [600], [513], 4, 4),
+                                               (80, [1000, 5, 400], [700, 900, 0], 2, 2)])
+def test_long_sequences(dtype, d, q_len, k_len, h, hk):
+    rng = np.random.default_rng(d)
+    check(rng, q_len, k_len, h, hk, d, dtype, gap_q=1, gap_k=2)
+    check(rng, q_len, k_len, h, hk, d, dtype, gap_q=1, gap_k=2, size=6.0)   # weights near one-hot
+
+
+@gpu
+def test_long_sequences_with_masks():
+    rng = np.random.default_rng(3)
+    check(rng, [300, 300], [400, 700], 2, 2, 64, "bf16", mask=0.5)
+
+
+@gpu
+def test_split_keys_take_a_workspace_and_small_calls_none():
+    rng = np.random.default_rng(2)
+    assert check(rng, [1], [4000], 1, 1, 64, "bf16") > 0
+    assert check(rng, [1] * 64, [64] * 64, 8, 8, 64, "bf16") == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_several_queries_share_one_source(dtype):
+    rng = np.random.default_rng(1)
+    q, k, v = typed(rng, (12, 4, 64), dtype), typed(rng, (50, 4, 64), dtype), typed(rng, (50, 4, 64), dtype)
+    q_start, q_len, k_start, k_len = [0, 5, 6], [5, 1, 6], [3, 3, 10], [40, 40, 33]
+    out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), q_start, q_len, k_start, k_len, dtype, 0.125)
+    compare(q, k, v, out, lse, q_start, q_len, k_start, k_len, dtype, 0.125)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_len", [1, 20, 300])
+def test_strides_and_head_major_layouts(dtype, q_len):
+    rng = np.random.default_rng(q_len)
+    h, d, n = 4, 64, 150
+    q = typed(rng, (h, q_len, d), dtype).cuda().transpose(0, 1)          # head-major
+    kv = typed(rng, (n, 2, h, d), dtype).cuda()                          # interleaved
+    wide = torch.full((q_len, h, d + 16), 7.0, dtype=q.dtype, device="cuda")
+    args = ([0], [q_len], [0], [n], dtype, 0.125)
+    a, la, _ = run(q.contiguous(), kv[:, 0].contiguous(), kv[:, 1].contiguous(), *args)
+    b, lb, _ = run(q, kv[:, 0], kv[:, 1], *args, out=wide[:, :, :d])
+    assert torch.equal(a, b) and torch.equal(la, lb) and bool((wide[:, :, d:] == 7).all())
+    # one key/value row for every head (stride 0)
+    one = kv[:, 0, :1].expand(n, h, d)
+    c, _, _ = run(q, one, one, *args)
+    e, _, _ = run(q.contiguous(), one.contiguous(), one.contiguous(), *args)
+    assert torch.equal(c, e)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_a_nan_query_spoils_its_own_row_only(dtype):
+    rng = np.random.default_rng(7)
+    for q_len in (4, 40, 200):
+        q, k, v = typed(rng, (q_len, 2, 64), dtype), typed(rng, (90, 2, 64), dtype), typed(rng, (90, 2, 64), dtype)
+        args = ([0], [q_len], [0], [90], dtype, 0.125)
+        good, gl, _ = run(q.cuda(), k.cuda(), v.cuda(), *args)
+        q[2, 1, 3] = float("nan")
+        out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), *args)
+        same = torch.ones(q_len, 2, dtype=torch.bool, device="cuda")
+        same[2, 1] = False
+        assert torch.equal(out[same], good[same]) and torch.equal(lse[same], gl[same])
+        assert bool(out[2, 1].isnan().all()) and bool(lse[2, 1].isnan())
+
+
+@gpu
+@pytest.mark.parametrize("q_len", [1, 200])
+def test_scores_far_from_zero(q_len):
+    # every score near +-4000 (f32 keeps 2^-12 of those): the maximum has to follow
+    rng = np.random.default_rng(9)
+    for sign in (1.0, -1.0):
+        q = torch.full((q_len, 1, 64), 2.0).to(torch.bfloat16)
+        k = (torch.full((100, 1, 64), 250.0 * sign)).to(torch.bfloat16)
+        v = typed(rng, (100, 1, 64), "bf16")
+        out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), [0], [q_len], [0], [100], "bf16", 0.125)
+        want = f64(v).mean(0)
+        np.testing.assert_allclose(f64(out), np.broadcast_to(want, out.shape), atol=2.0 ** -8 * np.abs(f64(v)).max())
+        np.testing.assert_allclose(f64(lse), 4000.0 * sign + np.log(100.0), rtol=2.0 ** -20)
+
+
+@gpu
+@pytest.mark.parametrize("field,value", [("q_start", -1), ("q_start", 9), ("q_len", -1), ("q_len", 4), ("k_start", -1),
+                                         ("k_start", 12), ("k_len", 21), ("k_len", -5), ("k_start", 2147483647)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_bad_lengths_are_left_out_and_reported(dtype, field, value):
+    rng = np.random.default_rng(4)
+    q, k, v = (typed(rng, (n, 2, 64), dtype).cuda() for n in (10, 30, 30))
+    given = {"q_start": [0, 5], "q_len": [3, 3], "k_start": [0, 10], "k_len": [20, 20]}
+    good, gl, _ = run(q, k, v, *given.values(), dtype, 0.125, max_q=3, max_k=20)
+    assert status_bits() == 0
+    given[field] = [value, given[field][1]]
+    out, lse, _ = run(q, k, v, *given.values(), dtype, 0.125, max_q=3, max_k=20)
+    assert status_bits() == 4
+    assert torch.equal(out[5:8], good[5:8]) and torch.equal(lse[5:8], gl[5:8])
+    rest = [i for i in range(10) if not 5 <= i < 8]
+    assert bool((out[rest] == 7).all()) and bool((lse[rest] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype,q_len,k_len", [("f32", 1, 900), ("bf16", 1, 2000), ("bf16", 300, 500), ("f16", 20, 90)])
+def test_captured_and_replayed_on_new_rows(dtype, q_len, k_len):
+    lib, rng = L.load(), np.random.default_rng(11)
+    q, k, v = (torch.zeros(n, 2, 64, dtype=DTYPES[dtype][0], device="cuda") for n in (q_len, k_len, k_len))
+    out, lse = torch.zeros_like(q), torch.zeros(q_len, 2, device="cuda")
+    a, _ = arguments(q, k, v, out, lse, [ints([0]), ints([q_len]), ints([0]), ints([k_len])], None, dtype, 0.125, q_len, k_len)
+    run(q, k, v, [0], [q_len], [0], [k_len], dtype, 0.125)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        assert lib.mc_cross_attention(C.byref(a), side.cuda_stream) == L.MC_OK
+    for _ in range(3):
+        for x in (q, k, v):
+            x.copy_(typed(rng, tuple(x.shape), dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, wl, _ = run(q, k, v, [0], [q_len], [0], [k_len], dtype, 0.125)
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+    # lse may be left out
+    a.lse = None
+    assert lib.mc_cross_attention(C.byref(a), None) == L.MC_OK
+
+
+@gpu
+def test_rows_past_2_gib():
+    # keys whose byte offsets pass 2^32, the sequence's the last of them
+    rng = np.random.default_rng(5)
+    rows, hk, d = 300_000, 64, 128     # 16 KiB a row: 4.6 GiB
+    k = torch.empty(rows, hk, d, dtype=torch.bfloat16, device="cuda")
+    n = 70
+    for q_len in (1, 140):
+        q = typed(rng, (q_len, hk, d), "bf16")
+        kv = typed(rng, (n, hk, d), "bf16")
+        k[rows - n:] = kv.cuda()
+        out, lse, _ = run(q.cuda(), k, k, [0], [q_len], [rows - n], [n], "bf16", d ** -0.5)
+        compare(q, kv, kv, out, lse, [0], [q_len], [0], [n], "bf16", d ** -0.5)
