@@ -64,7 +64,10 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 constexpr uint32_t kKeyNone = 0x007FFFFFu;  // key_of(-inf): a token that cannot be drawn
-constexpr int kList = 2048;                 // candidates that one CTA sorts
+constexpr int kCoarse = 512;                // bins of the histogram of counts
+constexpr int kList = 2048;                 // candidates that one CTA takes
+constexpr int kWarpList = 256;              // candidates that one warp takes
+constexpr int kCrowd = 64;                  // tokens of one bin beyond which comparing all pairs costs more than a sort
 // Weights vanish 42 halvings below the top: (top - v) / T above 42 ln 2.
 constexpr float kReach = 29.2f;
 
@@ -101,11 +104,10 @@ struct Weigher {
 
   // w = 2^-((top - v) rate) in [0, 1]: 2^-(k / 64) from the table times the
   // exponential series of the rest, |rest| <= ln 2 / 128, to its fourth
-  // power (the fifth is below 4e-14).  0 below 2^-42.
-  __device__ __forceinline__ double real(float v, uint32_t key) const {
-    if (key == top_key) return 1.0;
+  // power (the fifth is below 4e-14).  For 0 <= (top - v) rate < 1000, without a
+  // branch, so that several are in flight.
+  __device__ __forceinline__ double near(float v) const {
     const double y = __dmul_rn(__dsub_rn(top, widen(v)), rate);
-    if (!(y < 42.0)) return 0.0;
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
     const double t = __fma_rn(y, 64.0, magic);
     const int k = __double2loint(t);
@@ -117,6 +119,12 @@ struct Weigher {
     s = __fma_rn(s, z, 1.0);
     const double p = __dmul_rn(powers[k & 63], s);
     return __hiloint2double(__double2hiint(p) - ((k >> 6) << 20), __double2loint(p));
+  }
+  // Any v: 0 below 2^-42, 1 at the top even where top or rate is infinite.
+  __device__ __forceinline__ double real(float v, uint32_t key) const {
+    if (key == top_key) return 1.0;
+    if (!(__dmul_rn(__dsub_rn(top, widen(v)), rate) < 42.0)) return 0.0;
+    return near(v);
   }
   static __device__ __forceinline__ unsigned long long fixed(double w) {
     // adding 2^12 leaves the 40 fraction bits at the end of the mantissa
@@ -135,8 +143,9 @@ struct Shared {
     unsigned long long hist[2][kBins];  // the general way
     unsigned long long list[kList];     // candidates: key, then ~id
   };
-  uint32_t counts[kBins];
-  uint32_t listed;
+  uint32_t counts[kCoarse];      // tokens per bin of this CTA's slice
+  uint32_t starts[kCoarse + 1];  // of the whole row, up to each bin
+  uint32_t filled[kCoarse];      // candidates that have arrived in this CTA's list
   double powers[64];
   Exchange out;
   unsigned long long warp_value[kWarps];
@@ -201,6 +210,19 @@ struct Row {
       v = MAX ? (o > v ? o : v) : v + o;
     }
     return v;
+  }
+  // The largest of two values over the block, in one exchange.
+  __device__ __forceinline__ void block_max2(uint32_t& a, uint32_t& b) {
+    a = __reduce_max_sync(kFull, a);
+    b = __reduce_max_sync(kFull, b);
+    if (lane == 0) sh.warp_value[warp] = (unsigned long long)a << 32 | b;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const unsigned long long o = sh.warp_value[w];
+      a = max(a, (uint32_t)(o >> 32));
+      b = max(b, (uint32_t)o);
+    }
   }
   // Publishes this CTA's values; afterwards peer(r, i) reads those of CTA r.
   __device__ __forceinline__ void publish(unsigned long long a, unsigned long long b, unsigned long long c) {
@@ -326,6 +348,7 @@ struct Row {
   __device__ __forceinline__ unsigned long long segment_sum(F f) {
     unsigned long long s = 0;
     const int begin = warp * p.segment, end = min(n, begin + p.segment);
+#pragma unroll 4
     for (int i = begin + lane; i < end; i += 32) {
       const float v = at(i);
       s += f(v, key_of(v), base + i);
@@ -409,6 +432,178 @@ __device__ void sort_list(unsigned long long* list, int n2, int tid) {
   __syncthreads();
 }
 
+// Puts list[0, n) in the row's order.  The candidates arrived bin by bin, so
+// each takes its place among its bin's; a crowded bin makes that cost more
+// than sorting them all.
+template <int THREADS, typename F>
+__device__ void order_list(Shared& sh, int n, uint32_t at0, bool crowded, int tid, F bin_of_key) {
+  if (crowded) {
+    int n2 = 64;
+    while (n2 < n) n2 <<= 1;
+    for (int i = n + tid; i < n2; i += THREADS) sh.list[i] = 0;
+    __syncthreads();
+    sort_list(sh.list, n2, tid);
+    return;
+  }
+  constexpr int kEach = (THREADS == 32 ? kWarpList : kList) / THREADS;
+  unsigned long long own[kEach];
+  uint32_t place[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = tid + j * THREADS;
+    if (i >= n) break;
+    own[j] = sh.list[i];
+    const uint32_t bin = bin_of_key((uint32_t)(own[j] >> 32));
+    const uint32_t from = sh.starts[bin] - at0, to = sh.starts[bin + 1] - at0;
+    uint32_t ahead = 0;
+    for (uint32_t k = from; k < to; ++k) ahead += sh.list[k] > own[j];
+    place[j] = from + ahead;
+  }
+  if (THREADS == 32) __syncwarp(); else __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (tid + j * THREADS >= n) break;
+    sh.list[place[j]] = own[j];
+  }
+  if (THREADS == 32) __syncwarp(); else __syncthreads();
+}
+
+struct Cuts {
+  bool by_k, by_p;
+  int top_k;
+  double top_p, floor_w, u;
+  unsigned long long whole, ahead;  // weights of the row, and before the list
+  bool border_only;                 // the list is about top_p's border: find that
+};
+
+// The cuts and the draw from the ordered list, by one warp or by the block.
+// Returns 1 when the token is drawn, 0 when the list does not reach top_p's
+// border, or the last candidate that top_p keeps (border_only).
+template <typename T, bool WARP>
+__device__ unsigned long long finish_list(Row<T>& r, const Weigher& weigh, const Cuts& q, int listed) {
+  Shared& sh = r.sh;
+  constexpr int kEach = (WARP ? kWarpList : kList) / (WARP ? 32 : kThreads);
+  const int tid = r.tid, lane = r.lane, first = tid * kEach;
+  auto total_of = [&](unsigned long long v) { return WARP ? warp_sum(v) : r.template block<false>(v); };
+  // thread i holds the ordered candidates kEach i .. kEach i + kEach - 1
+  const int in_a = q.by_k ? min(listed, q.top_k) : listed;
+  unsigned long long weight[kEach], sum = 0;
+  uint32_t above_floor = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    weight[j] = 0;
+    if (first + j < in_a) {
+      const double real = weigh.near(value_of((uint32_t)(sh.list[first + j] >> 32)));
+      weight[j] = Weigher::fixed(real);
+      above_floor += real >= q.floor_w;
+    }
+    sum += weight[j];
+  }
+  int in_c = in_a;
+  if (q.by_p) {
+    unsigned long long run = warp_prefix(sum, lane) - sum, all;
+    if (WARP) {
+      all = __shfl_sync(kFull, run + sum, 31);
+    } else {
+      __syncthreads();
+      if (lane == 31) sh.warp_value[r.warp] = run + sum;
+      __syncthreads();
+      all = 0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < r.warp) run += sh.warp_value[i];
+        all += sh.warp_value[i];
+      }
+    }
+    const unsigned long long mass_a = q.by_k ? all : q.whole;
+    unsigned long long border = (unsigned long long)ceil(__dmul_rn(q.top_p, (double)mass_a));
+    border = border < 1 ? 1 : border > mass_a ? mass_a : border;
+    if (q.ahead >= border || q.ahead + all < border) return 0;
+    border -= q.ahead;
+    // those whose running sum before them is below the border
+    uint32_t below = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      below += first + j < in_a && run < border;
+      run += weight[j];
+    }
+    in_c = (int)total_of(below);
+    if (q.border_only) return sh.list[in_c - 1];
+  }
+  in_c = min(in_c, (int)total_of(above_floor));
+  sum = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (first + j >= in_c) weight[j] = 0;
+    sum += weight[j];
+  }
+  const unsigned long long total = total_of(sum);
+  unsigned long long target = (unsigned long long)floor(__dmul_rn(q.u, (double)total));
+  if (target >= total) target = total - 1;
+  uint32_t drawn = 0;
+  unsigned long long drawn_weight = 0;
+  if (WARP) {
+    // The lowest id at which the weights up to it exceed target, by halving.
+    uint32_t id[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) id[j] = weight[j] ? kFull - (uint32_t)sh.list[first + j] : kFull;
+    uint32_t lo = 0, hi = (uint32_t)r.p.vocab - 1;
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) >> 1;
+      unsigned long long s = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) s += id[j] <= mid ? weight[j] : 0ull;
+      if (warp_sum(s) > target)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    drawn = lo;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) drawn_weight += id[j] == drawn ? weight[j] : 0ull;
+    drawn_weight = warp_sum(drawn_weight);
+  } else {
+    // The same, 256 ranges of ids at a time, by their weights.
+    unsigned long long* ranges = reinterpret_cast<unsigned long long*>(sh.counts);
+    static_assert(sizeof(sh.counts) >= kThreads * sizeof(unsigned long long), "a range per thread");
+    for (int shift = max(0, 32 - 8 - __clz((uint32_t)r.p.vocab));; shift = max(0, shift - 8)) {
+      __syncthreads();
+      ranges[tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (weight[j]) {
+          const uint32_t id = kFull - (uint32_t)sh.list[first + j], at = (id - drawn) >> shift;
+          if (id >= drawn && at < 256) atomicAdd(&ranges[at], weight[j]);
+        }
+      __syncthreads();
+      const unsigned long long mine = ranges[tid], inc = warp_prefix(mine, lane);
+      if (lane == 31) sh.warp_value[r.warp] = inc;
+      __syncthreads();
+      unsigned long long start = inc - mine;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i)
+        if (i < r.warp) start += sh.warp_value[i];
+      if (start <= target && target < start + mine) {
+        sh.found[0] = tid;
+        sh.found[1] = start;
+        sh.found[2] = mine;
+      }
+      __syncthreads();
+      drawn += (uint32_t)sh.found[0] << shift;
+      target -= sh.found[1];
+      drawn_weight = sh.found[2];
+      if (shift == 0) break;
+    }
+  }
+  if (tid == 0) {
+    const int row = blockIdx.x / r.ranks;
+    r.p.tokens[row] = (int32_t)drawn;
+    if (r.p.probs) r.p.probs[row] = (float)__ddiv_rn((double)drawn_weight, (double)total);
+  }
+  return 1;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t dyn[];
@@ -419,8 +614,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   const int row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31;
   const int slice = p.segment * kWarps, base = min(p.vocab, rank * slice), n = min(slice, p.vocab - base);
   if (tid < 64) sh.powers[tid] = exp2(-(double)tid / 64.0);
-  if (tid == 0) sh.listed = 0;
-  for (int i = tid; i < kBins; i += kThreads) sh.counts[i] = 0;
+  for (int i = tid; i < kCoarse; i += kThreads) sh.counts[i] = sh.filled[i] = 0;
   pdl_enter();
 
   // ---- the logits, once ----
@@ -468,7 +662,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
 
   Row<T> r{p, sh, x, cluster, ranks, rank, base, n, tid, lane, tid >> 5, 0, 0};
   {
-    const unsigned long long a = r.template block<true>(key_of(most)), b = r.template block<true>(~key_of(least) & kFull);
+    uint32_t a = key_of(most), b = ~key_of(least);
+    r.block_max2(a, b);
     r.publish(a, b, 0);
   }
   unsigned long long top_bits = 0, least_bits = 0;
@@ -514,239 +709,149 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0f;
 
   // ---- the few that matter, in one CTA ----
+  Cut cut{kKeyNone, -1};
+  bool cut_found = false;
   if ((by_k || by_p || floor_w > 0.0) && range > 0.0f && range < 1e30f && top < INFINITY) {
-    // bin = round(step (top - v)) + 1 or so: the sum of a constant, v times
+    // bin = round(step (top - v) + 2 or so): the sum of a constant, v times
     // -step and 1.5 * 2^23, whose last bits are the rounded whole number; it
-    // never decreases as v falls.  NaN and what lies out of reach end above kBins.
-    const float step = __fdiv_rn((float)(kBins - 8), range);
+    // never decreases as v falls.  NaN and what lies out of reach end above kCoarse.
+    const float step = __fdiv_rn((float)(kCoarse - 8), range);
     const float origin = __fadd_rn(__fmul_rn(top, step), 12582912.0f + 2.0f);
-    const bool binned = __fmul_rn(fabsf(top), step) < 4194304.0f;  // else the constant loses the bins
-    if (binned) {
+    if (__fmul_rn(fabsf(top), step) < 4194304.0f) {  // else the constant loses the bins
+      const float lead = __fmaf_rn(-top, step, __fsub_rn(origin, 12582912.0f));  // the top's place, about 2
       auto bin_of = [&](float v) { return __float_as_uint(__fmaf_rn(v, -step, origin)) - 0x4B400000u; };
-      unsigned long long whole = 0;
       const bool need_whole = by_p && !by_k;
+      unsigned long long whole = 0;
       if (need_whole) {
         each([&](float v, int) {
           const uint32_t b = bin_of(v);
-          if (b >= kBins) return;
-          atomicAdd(&sh.counts[b], 1u);
-          v = __fadd_rn(v, 0.0f);
-          whole += Weigher::fixed(weigh.real(v, key_of(v)));
+          const unsigned long long w = Weigher::fixed(weigh.near(v));
+          if (b < kCoarse) {
+            atomicAdd(&sh.counts[b], 1u);
+            whole += w;
+          }
         });
         whole = r.template block<false>(whole);
       } else {
         each([&](float v, int) {
           const uint32_t b = bin_of(v);
-          if (b < kBins) atomicAdd(&sh.counts[b], 1u);
+          if (b < kCoarse) atomicAdd(&sh.counts[b], 1u);
         });
       }
       __syncthreads();
       r.publish(whole, 0, 0);
-      constexpr int kPer = kBins / kThreads;
-      static_assert(kPer == 4, "a thread's bins are one 16-byte load");
-      uint32_t c[kPer] = {0, 0, 0, 0};
+      static_assert(kCoarse == 2 * kThreads, "a thread has two bins");
+      uint32_t c0 = 0, c1 = 0;
       whole = 0;
       for (int i = 0; i < ranks; ++i) {
-        const uint4 o = reinterpret_cast<const uint4*>(cluster.map_shared_rank(&sh, i)->counts)[tid];
-        c[0] += o.x;
-        c[1] += o.y;
-        c[2] += o.z;
-        c[3] += o.w;
+        const uint2 o = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&sh, i)->counts)[tid];
+        c0 += o.x;
+        c1 += o.y;
         whole += r.peer(i, 0);
       }
-      // Counts and estimated weights up to each bin.
+      // Counts and estimated weights up to each bin, both in one scan.
       const float bits = __fdiv_rn((float)weigh.rate, step);  // halvings per bin
-      float w[kPer];
-      uint32_t count = 0;
-      float mass = 0.0f;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        w[j] = __fmul_rn((float)c[j], exp2f(__fmul_rn(-bits, (float)(tid * kPer + j - 2))));
-        count += c[j];
-        mass = __fadd_rn(mass, w[j]);
-      }
-      // both prefixes of the block in one scan: the count above, the estimate
-      // (f32 bits) beside it
-      uint32_t count_in = count;
-      float mass_in = mass;
+      const int bin0 = 2 * tid;
+      const float w0 = __fmul_rn((float)c0, exp2_approx(__fmul_rn(bits, __fsub_rn(lead, (float)bin0))));
+      const float w1 = __fmul_rn((float)c1, exp2_approx(__fmul_rn(bits, __fsub_rn(lead, (float)(bin0 + 1)))));
+      uint32_t count = c0 + c1;
+      float mass = __fadd_rn(w0, w1);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t a = __shfl_up_sync(kFull, count_in, o);
-        const float b = __shfl_up_sync(kFull, mass_in, o);
+        const uint32_t a = __shfl_up_sync(kFull, count, o);
+        const float b = __shfl_up_sync(kFull, mass, o);
         if (lane >= o) {
-          count_in += a;
-          mass_in = __fadd_rn(mass_in, b);
+          count += a;
+          mass = __fadd_rn(mass, b);
         }
       }
-      if (lane == 31)
-        sh.warp_value[tid >> 5] = (unsigned long long)count_in << 32 | __float_as_uint(mass_in);
-      if (tid == 0) sh.found[0] = kBins;
+      if (lane == 31) sh.warp_value[tid >> 5] = (unsigned long long)count << 32 | __float_as_uint(mass);
+      if (tid == 0) sh.found[0] = sh.found[1] = kCoarse - 1;
       __syncthreads();
-      uint32_t before = count_in - count, total = 0;
-      float mass_before = __fsub_rn(mass_in, mass), mass_total = 0.0f;
+      float mass_total = 0.0f;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
         const unsigned long long o = sh.warp_value[i];
         if (i < (tid >> 5)) {
-          before += (uint32_t)(o >> 32);
-          mass_before = __fadd_rn(mass_before, __uint_as_float((uint32_t)o));
+          count += (uint32_t)(o >> 32);
+          mass = __fadd_rn(mass, __uint_as_float((uint32_t)o));
         }
-        total += (uint32_t)(o >> 32);
         mass_total = __fadd_rn(mass_total, __uint_as_float((uint32_t)o));
       }
-      // The last bin that can matter: the first that satisfies any of the cuts.
-      const float want = __fmul_rn(__fadd_rn(fmaxf(top_p, 0.0f), 0.01f), mass_total);
+      sh.starts[bin0] = count - c0 - c1;
+      sh.starts[bin0 + 1] = count - c1;
+      if (tid == kThreads - 1) sh.starts[kCoarse] = count;
+      // The last bin that can matter: the first that satisfies any of the
+      // cuts.  For a top_p of many tokens also the first bin near its border.
+      const float share = fmaxf(top_p, 0.0f);
+      const float near_p = __fmul_rn(__fsub_rn(share, 0.005f), mass_total), past_p = __fmul_rn(__fadd_rn(share, 0.01f), mass_total);
       const float floor_bin = floor_w > 0.0 ? __fadd_rn(__fdiv_rn(-log2f((float)floor_w), bits), 6.0f) : 1e30f;
-      uint32_t last = kBins;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int bin = tid * kPer + j;
-        before += c[j];
-        mass_before = __fadd_rn(mass_before, w[j]);
-        const bool enough = (by_k && before >= (uint32_t)top_k) || (need_whole && mass_before >= want) ||
-                            (!by_p && (float)bin >= floor_bin);
-        if (enough && last == kBins) last = bin;
-      }
-      atomicMin(reinterpret_cast<unsigned long long*>(&sh.found[0]), (unsigned long long)last);
+      auto enough = [&](int bin, uint32_t c, float m) {
+        return (by_k && c >= (uint32_t)top_k) || (need_whole && m >= past_p) || (!by_p && (float)bin >= floor_bin);
+      };
+      if (enough(bin0, count - c1, __fsub_rn(mass, w1)))
+        atomicMin(&sh.found[0], (unsigned long long)bin0);
+      else if (enough(bin0 + 1, count, mass))
+        atomicMin(&sh.found[0], (unsigned long long)(bin0 + 1));
+      if (need_whole && mass >= near_p) atomicMin(&sh.found[1], (unsigned long long)bin0);
       __syncthreads();
-      last = min((uint32_t)sh.found[0], (uint32_t)kBins - 1);
-      // how many tokens lie up to it
-      if (tid == (int)last / kPer) {
-        uint32_t up_to = before;
-#pragma unroll
-        for (int j = kPer - 1; j >= 0; --j)
-          if (tid * kPer + j > (int)last) up_to -= c[j];
-        sh.found[1] = up_to;
-      }
-      __syncthreads();
-      const uint32_t listed = (uint32_t)sh.found[1];
+      const uint32_t last = (uint32_t)sh.found[0];
+      const bool crowded = __syncthreads_or((bin0 <= (int)last && c0 > kCrowd) || (bin0 + 1 <= (int)last && c1 > kCrowd));
+      // All candidates, or, where they are too many, those about top_p's border.
+      uint32_t from = 0;
+      if (sh.starts[last + 1] > kList && need_whole) from = (uint32_t)min(sh.found[1], sh.found[0]);
+      const uint32_t at0 = sh.starts[from], listed = sh.starts[last + 1] - at0;
       if (listed <= kList) {
         Shared* home = cluster.map_shared_rank(&sh, 0);
+        unsigned long long ahead = 0;  // the weights before the list
         each([&](float v, int i) {
-          if (bin_of(v) > last) return;
-          const uint32_t slot = atomicAdd(&home->listed, 1u);
+          const uint32_t b = bin_of(v);
+          if (b > last) return;
           v = __fadd_rn(v, 0.0f);
+          if (b < from) {
+            ahead += Weigher::fixed(weigh.near(v));
+            return;
+          }
+          const uint32_t slot = sh.starts[b] - at0 + atomicAdd(&home->filled[b], 1u);
           if (slot < kList) home->list[slot] = (unsigned long long)key_of(v) << 32 | (kFull - (uint32_t)(base + i));
         });
-        cluster.sync();
-        int done = 0;
-        if (rank == 0) {
-          int n2 = 64;
-          while (n2 < (int)listed) n2 <<= 1;
-          for (int i = listed + tid; i < n2; i += kThreads) sh.list[i] = 0;
-          __syncthreads();
-          sort_list(sh.list, n2, tid);
-          // thread i holds the sorted candidates kEach i .. kEach i + kEach - 1
-          constexpr int kEach = kList / kThreads;
-          const int first = tid * kEach;
-          unsigned long long weight[kEach], sum = 0;
-          uint32_t above_floor = 0;
-          const int in_a = by_k ? min((int)listed, top_k) : (int)listed;
-#pragma unroll
-          for (int j = 0; j < kEach; ++j) {
-            weight[j] = 0;
-            if (first + j < in_a) {
-              const uint32_t k = (uint32_t)(sh.list[first + j] >> 32);
-              const double real = weigh.real(value_of(k), k);
-              weight[j] = Weigher::fixed(real);
-              above_floor += real >= floor_w;
-            }
-            sum += weight[j];
-          }
-          const unsigned long long in = warp_prefix(sum, lane);
-          __syncthreads();
-          if (lane == 31) sh.warp_value[tid >> 5] = in;
-          __syncthreads();
-          unsigned long long run = in - sum, all = 0;
-#pragma unroll
-          for (int i = 0; i < kWarps; ++i) {
-            if (i < (tid >> 5)) run += sh.warp_value[i];
-            all += sh.warp_value[i];
-          }
-          int in_c = in_a;
-          bool covered = true;
-          if (by_p) {
-            const unsigned long long mass_a = by_k ? all : whole;
-            unsigned long long border = (unsigned long long)ceil(__dmul_rn(fmax((double)top_p, 0.0), (double)mass_a));
-            border = border < 1 ? 1 : border > mass_a ? mass_a : border;
-            covered = all >= border;
-            // those whose running sum before them is below the border
-            uint32_t below = 0;
-            unsigned long long s = run;
-#pragma unroll
-            for (int j = 0; j < kEach; ++j) {
-              below += first + j < in_a && s < border;
-              s += weight[j];
-            }
-            in_c = (int)r.template block<false>(below);
-          }
-          if (covered) {
-            done = 1;
-            in_c = min(in_c, (int)r.template block<false>(above_floor));
-            sum = 0;
-#pragma unroll
-            for (int j = 0; j < kEach; ++j) {
-              if (first + j >= in_c) weight[j] = 0;
-              sum += weight[j];
-            }
-            const unsigned long long total_c = r.template block<false>(sum);
-            unsigned long long target = (unsigned long long)floor(__dmul_rn(u, (double)total_c));
-            if (target >= total_c) target = total_c - 1;
-            // The first id at which the running sum passes target: 256 ranges
-            // of ids at a time, by their weights.
-            uint32_t from = 0;
-            int shift = max(0, 32 - 8 - __clz((uint32_t)p.vocab));
-            unsigned long long drawn = 0;
-            for (;; shift = max(0, shift - 8)) {
-              unsigned long long* ranges = reinterpret_cast<unsigned long long*>(sh.counts);  // 256 of them
-              ranges[tid] = 0;
-              __syncthreads();
-#pragma unroll
-              for (int j = 0; j < kEach; ++j)
-                if (weight[j]) {
-                  const uint32_t id = kFull - (uint32_t)sh.list[first + j];
-                  const uint32_t at = (id - from) >> shift;
-                  if (id >= from && at < 256) atomicAdd(&ranges[at], weight[j]);
-                }
-              __syncthreads();
-              const unsigned long long mine = ranges[tid], inc = warp_prefix(mine, lane);
-              if (lane == 31) sh.warp_value[tid >> 5] = inc;
-              __syncthreads();
-              unsigned long long start = inc - mine;
-#pragma unroll
-              for (int i = 0; i < kWarps; ++i)
-                if (i < (tid >> 5)) start += sh.warp_value[i];
-              if (start <= target && target < start + mine) {
-                sh.found[0] = tid;
-                sh.found[1] = start;
-                sh.found[2] = mine;
-              }
-              __syncthreads();
-              from += (uint32_t)sh.found[0] << shift;
-              target -= sh.found[1];
-              drawn = sh.found[2];
-              __syncthreads();
-              if (shift == 0) break;
-            }
-            if (tid == 0) {
-              p.tokens[row] = (int32_t)from;
-              if (p.probs) p.probs[row] = (float)__ddiv_rn((double)drawn, (double)total_c);
-            }
+        if (from) ahead = r.template block<false>(ahead);
+        r.publish(ahead, 0, 0);  // and the list is complete
+        unsigned long long outcome = 0;
+        if (rank == 0 && (listed > kWarpList || crowded || from || tid < 32)) {
+          ahead = 0;
+          if (from)
+            for (int i = 0; i < ranks; ++i) ahead += r.peer(i, 0);
+          const Cuts cuts{by_k, by_p, top_k, fmax((double)top_p, 0.0), floor_w, u, whole, ahead, from > 0};
+          auto value_bin = [&](uint32_t key) { return bin_of(value_of(key)); };
+          if (listed > kWarpList || crowded || from) {
+            order_list<kThreads>(sh, (int)listed, at0, crowded, tid, value_bin);
+            outcome = finish_list<T, false>(r, weigh, cuts, (int)listed);
+          } else {
+            order_list<32>(sh, (int)listed, at0, false, tid, value_bin);
+            outcome = finish_list<T, true>(r, weigh, cuts, (int)listed);
           }
         }
-        if (!need_whole) return;  // nothing was estimated: the list holds every cut
-        // every CTA learns whether the list reached top_p's border
-        r.publish(done, 0, 0);
-        done = (int)r.peer(0, 0);
-        cluster.sync();
-        if (done) return;
+        if (!need_whole) return;  // nothing was estimated: the list held every cut
+        // Every CTA learns whether the list reached top_p's border: 1 = drawn,
+        // more = the cut, for a draw from all.
+        r.publish(outcome, 0, 0);
+        outcome = r.peer(0, 0);
+        if (outcome == 1) {
+          cluster.sync();  // no CTA leaves while another may read its shared memory
+          return;
+        }
+        if (outcome) {
+          cut.key = (uint32_t)(outcome >> 32);
+          cut.last = (int)(kFull - (uint32_t)outcome);
+          cut_found = true;
+        }
       }
     }
   }
 
   // ---- the general way: top-k, then top-p ----
   const uint32_t key_min = max(kKeyNone + 1, key_of(__fsub_rn(top, __fmul_rn(kReach, temperature))));
-  Cut cut{kKeyNone, -1};
   unsigned long long above, ties, whole;
   if (by_k) {
     auto one = [](float, uint32_t) -> unsigned long long { return 1; };
@@ -757,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       cut.key = key;
     }
   }
-  if (by_p) {
+  if (by_p && !cut_found) {
     auto mass = [&](float v, uint32_t k) { return Weigher::fixed(weigh.real(v, k)); };
     const uint32_t key = r.border(cut, mass, 0, top, range, max(key_min, cut.key), key_max, &above, &ties, &whole,
                                   fmax((double)top_p, 0.0));
