@@ -10,13 +10,23 @@
 // One cluster of CTAs per row: each keeps a slice of the logits in shared
 // memory, so they are read from HBM once, and every later pass runs there.
 // The row is not sorted.  One histogram of counts, linear in the logits, says
-// above which bin all that can matter lies (the k-th logit, an estimate of
-// top_p's border, min_p's floor); those tokens, seldom more than a few hundred, go
-// to one CTA, which sorts them and finds the three cuts and the draw exactly.
-// A row whose candidates do not fit its list, or whose estimate turns out too
-// small, takes the general way: the border of a prefix of the order is "above
-// a key, and so many ties of it", and histograms narrow the key's range,
-// linear in the logits first and in their bit patterns from then on.
+// above which bin all that can matter lies (the k-th logit, top_p's border by
+// the bins' smallest weights, min_p's floor); those tokens, seldom more than a
+// few hundred, go to one CTA, of which one warp (or all, for more than 256)
+// orders them and finds the three cuts and the draw exactly, while the other
+// CTAs are done.  Without cuts, the draw is the place of u times the sum of
+// all weights, in the part of the row that holds it.
+//
+// Rows with more candidates than the list takes go the general way: each cut
+// is the border of a prefix of the order, "above a key, and so many ties of
+// it"; a histogram of exact weights or counts finds the bin that it lies in,
+// whose tokens are sorted, and the draw is from all tokens before it.
+//
+// Measured at 1,024 x 32,000 f32, mixed settings, for other layouts: every
+// border by histograms of keys 587 us; three passes over L2 by one CTA per row
+// 225 us (L2 gives 17 bytes a cycle and SM there); one pass over HBM with a
+// sample's threshold 321 us, of which the few rows that the sample misjudges
+// are two thirds; slices of 16,384 or 4,096 logits 200 and 270 us.
 //
 // Weights are fixed-point integers, 40 fraction bits (a 64-bit sum holds
 // 2^24 of them): sums do not depend on their order, so neither atomics nor
@@ -38,7 +48,11 @@ namespace cg = cooperative_groups;
 constexpr uint32_t kFull = 0xFFFFFFFFu;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 1024;
+constexpr int kBins = 1024;                  // of the general way's histograms
+constexpr int kBinBits = 10;
+static_assert(kBins == 1 << kBinBits, "a bin is the leading bits of a key's place");
+constexpr int kThreadBits = 8;
+static_assert(kThreads == 1 << kThreadBits, "a thread is the leading bits of an id's place");
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 393216;  // as the lexical shortlist's masks (kernels.cuh)
 
@@ -66,6 +80,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 constexpr uint32_t kKeyNone = 0x007FFFFFu;  // key_of(-inf): a token that cannot be drawn
 constexpr int kCoarse = 512;                // bins of the histogram of counts
 constexpr int kList = 2048;                 // candidates that one CTA takes
+constexpr int kAhead = 2;                   // the largest logit's bin, about
 constexpr int kWarpList = 256;              // candidates that one warp takes
 constexpr int kCrowd = 64;                  // tokens of one bin beyond which comparing all pairs costs more than a sort
 // Weights vanish 42 halvings below the top: (top - v) / T above 42 ln 2.
@@ -98,33 +113,46 @@ __device__ __forceinline__ double widen(float v) {
 }
 
 struct Weigher {
-  double top, rate;      // the largest logit; log2(e) / T
+  double top, rate;      // the weight's logit of 1; log2(e) / T
   uint32_t top_key;
   const double* powers;  // 2^-(j / 64)
+  double per_step, origin, per_logit, shift;
 
-  // w = 2^-((top - v) rate) in [0, 1]: 2^-(k / 64) from the table times the
-  // exponential series of the rest, |rest| <= ln 2 / 128, to its fourth
-  // power (the fifth is below 4e-14).  For 0 <= (top - v) rate < 1000, without a
-  // branch, so that several are in flight.
-  __device__ __forceinline__ double near(float v) const {
-    const double y = __dmul_rn(__dsub_rn(top, widen(v)), rate);
-    const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-    const double t = __fma_rn(y, 64.0, magic);
+  __device__ __forceinline__ Weigher(float top_, double temperature, const double* powers_)
+      : top((double)top_), rate(1.4426950408889634074 / temperature), top_key(key_of(top_)), powers(powers_) {
+    per_step = rate * -64.0;
+    origin = 6755399441055744.0 - per_step * top;  // 1.5 * 2^52 more: the sum is rounded to a whole number
+    per_logit = 1.0 / temperature;
+    shift = -top * per_logit;
+  }
+  // w = exp((v - top) / T): with k near 64 rate (top - v), 2^-(k / 64) from the
+  // table times exp(z), z = (v - top) / T + k ln 2 / 64, |z| <= 0.011, by its
+  // series to the fifth power (the sixth is below 3e-15).  For
+  // |top - v| rate < 1000 and |top| rate < 2^42, without a branch, so that
+  // several are in flight; above the top, w is above 1.  Returned as a
+  // product, *rest times the result.
+  __device__ __forceinline__ double near(float v, double* rest) const {
+    const double x = widen(v), t = __fma_rn(x, per_step, origin);
     const int k = __double2loint(t);
-    const double r = __fma_rn(__dsub_rn(t, magic), 0.015625, -y);  // k / 64 - y
-    const double z = __dmul_rn(r, 0.69314718055994530942);
-    double s = __fma_rn(z, 1.0 / 24, 1.0 / 6);
+    const double z = __fma_rn(x, per_logit, __fma_rn(__dsub_rn(t, 6755399441055744.0), 0.010830424696249145, shift));
+    double s = __fma_rn(z, 1.0 / 120, 1.0 / 24);
+    s = __fma_rn(s, z, 1.0 / 6);
     s = __fma_rn(s, z, 0.5);
     s = __fma_rn(s, z, 1.0);
-    s = __fma_rn(s, z, 1.0);
-    const double p = __dmul_rn(powers[k & 63], s);
+    *rest = __fma_rn(s, z, 1.0);
+    const double p = powers[k & 63];
     return __hiloint2double(__double2hiint(p) - ((k >> 6) << 20), __double2loint(p));
   }
-  // Any v: 0 below 2^-42, 1 at the top even where top or rate is infinite.
-  __device__ __forceinline__ double real(float v, uint32_t key) const {
+  __device__ __forceinline__ double near(float v) const {
+    double rest;
+    const double p = near(v, &rest);
+    return __dmul_rn(p, rest);
+  }
+  // Any v, top and T: 0 below 2^-42, 1 at the top even where it or rate is infinite.
+  __device__ double real(float v, uint32_t key) const {
     if (key == top_key) return 1.0;
-    if (!(__dmul_rn(__dsub_rn(top, widen(v)), rate) < 42.0)) return 0.0;
-    return near(v);
+    const double y = __dmul_rn(__dsub_rn(top, (double)v), rate);
+    return y < 42.0 ? exp2(-y) : 0.0;
   }
   static __device__ __forceinline__ unsigned long long fixed(double w) {
     // adding 2^12 leaves the 40 fraction bits at the end of the mantissa
@@ -143,16 +171,18 @@ struct Shared {
     unsigned long long hist[2][kBins];  // the general way
     unsigned long long list[kList];     // candidates: key, then ~id
   };
-  uint32_t counts[kCoarse];      // tokens per bin of this CTA's slice
+  uint32_t counts[kCoarse];      // tokens per bin, of the sample, the list or the slice
   uint32_t starts[kCoarse + 1];  // of the whole row, up to each bin
-  uint32_t filled[kCoarse];      // candidates that have arrived in this CTA's list
+  uint32_t filled[kCoarse];      // candidates of each bin that have arrived
+  uint32_t listed;               // tokens of a border's bin
   double powers[64];
   Exchange out;
   unsigned long long warp_value[kWarps];
   unsigned long long found[3];
 };
 
-__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
+template <typename V>
+__device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
@@ -165,13 +195,35 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
   }
   return v;
 }
-__device__ __forceinline__ unsigned long long warp_prefix(unsigned long long v, int lane) {
+template <typename V>
+__device__ __forceinline__ V warp_prefix(V v, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long w = __shfl_up_sync(kFull, v, o);
+    const V w = __shfl_up_sync(kFull, v, o);
     if (lane >= o) v += w;
   }
   return v;
+}
+
+// Sorts list[0, 2^m) in descending order (bitonic).
+__device__ void sort_list(unsigned long long* list, int n2, int tid) {
+  for (int size = 2; size <= n2; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      for (int i = tid; i < n2 / 2; i += kThreads) {
+        const int a = 2 * i - (i & (step - 1)), b = a + step;
+        const unsigned long long u = list[a], v = list[b];
+        if ((u < v) == ((a & size) == 0)) {
+          list[a] = v;
+          list[b] = u;
+        }
+      }
+      // pairs up to 32 apart stay within one warp's 64 elements
+      if (step > 32 || (step == 1 && size >= 64))
+        __syncthreads();
+      else
+        __syncwarp();
+    }
+  __syncthreads();
 }
 
 // Which tokens are still in: those above `key`, and those equal to it with an
@@ -186,7 +238,7 @@ template <typename T>
 struct Row {
   const SampleParams& p;
   Shared& sh;
-  const T* x;  // this CTA's slice in shared memory
+  T* x;  // this CTA's slice in shared memory
   cg::cluster_group cluster;
   int ranks, rank, base, n, tid, lane, warp, turn, level;
 
@@ -194,6 +246,20 @@ struct Row {
   __device__ __forceinline__ float at(int i) const {
     const float v = Logit<T>::get(x[i]);
     return v == v ? __fadd_rn(v, 0.0f) : -INFINITY;
+  }
+  // One pass over the slice, each warp over its segment, 16 bytes at a time:
+  // f(logit, place).  The slice is padded with tokens that cannot be drawn.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    constexpr int kVec = 16 / (int)sizeof(T);
+    const int begin = min(n, warp * p.segment), end = min(n, begin + p.segment);
+    for (int i = begin + lane * kVec; i < end; i += 32 * kVec) {
+      const uint4 q = *reinterpret_cast<const uint4*>(x + i);
+      T t[kVec];
+      memcpy(t, &q, 16);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) f(Logit<T>::get(t[j]), i + j);
+    }
   }
 
   // ---- reductions over the row ----
@@ -215,6 +281,7 @@ struct Row {
   __device__ __forceinline__ void block_max2(uint32_t& a, uint32_t& b) {
     a = __reduce_max_sync(kFull, a);
     b = __reduce_max_sync(kFull, b);
+    __syncthreads();
     if (lane == 0) sh.warp_value[warp] = (unsigned long long)a << 32 | b;
     __syncthreads();
 #pragma unroll
@@ -239,48 +306,45 @@ struct Row {
   }
 
   // ---- the border of a prefix of the order ----
-  // The first key (descending) at which the sum of f over the tokens of `in`
-  // reaches target; *above is the sum over larger keys, *ties that over the
-  // key itself.  Returns 0 when the whole sum does not reach target.
+  // Cuts `cut` to the shortest prefix of the order (of the tokens it holds)
+  // whose sum of f reaches target, or `share` of the whole sum where that is
+  // not negative; leaves it alone when the whole sum does not reach target.
+  // A histogram linear in the logits finds the bin of the border; its tokens
+  // are sorted in CTA 0.  Where they are too many, histograms of the keys'
+  // leading bits narrow them down to one key, and its ties are counted.
   template <typename F>
-  __device__ uint32_t border(const Cut& in, F f, unsigned long long target, float top, float range, uint32_t key_min,
-                             uint32_t key_max, unsigned long long* above, unsigned long long* ties,
-                             unsigned long long* whole, double share) {
+  __device__ void border(Cut* cut, F f, unsigned long long target, float top, float range, uint32_t key_min,
+                         uint32_t key_max, double share) {
+    const Cut in = *cut;
     uint32_t lo = key_min, hi = key_max;
-    unsigned long long over = 0;
-    // A first histogram linear in the logits, where they are spread out; its
-    // bins are whole ranges of keys, as rounding keeps the order.
+    unsigned long long over = 0, ties = 0;
     const bool linear = range > 0.0f && range < INFINITY;
     const float step = linear ? __fdiv_rn((float)kBins * 0.999f, range) : 0.0f;
-    auto bin_of = [&](float v) {
-      return (int)fminf(__fmul_rn(__fsub_rn(top, v), step), (float)(kBins - 1));
+    // whole ranges of keys, as rounding keeps the order
+    auto bin_of = [&](float v) { return (int)fminf(__fmul_rn(__fsub_rn(top, v), step), (float)(kBins - 1)); };
+    auto held = [&](float& v, int i, uint32_t* k) {
+      v = v == v ? __fadd_rn(v, 0.0f) : -INFINITY;
+      *k = key_of(v);
+      return *k >= lo && *k <= hi && in.holds(*k, base + i);
     };
     int first_bin = -1;
     for (bool start = linear;; start = false) {
       unsigned long long* hist = sh.hist[level & 1];
       ++level;
+      __syncthreads();
       for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
       __syncthreads();
       int shift = 0;
       if (!start) {
         const uint32_t span = hi - lo;
-        shift = span < kBins ? 0 : 32 - 10 - __clz(span);
+        shift = span < kBins ? 0 : 32 - kBinBits - __clz(span);
       }
-      const int begin = warp * p.segment, end = min(n, begin + p.segment);
-      for (int i = begin + lane; i < end; i += 32) {
-        const float v = at(i);
-        const uint32_t k = key_of(v);
-        if (k < lo || k > hi || !in.holds(k, base + i)) continue;
-        int bin;
-        if (start) {
-          bin = bin_of(v);
-        } else {
-          if (first_bin >= 0 && bin_of(v) != first_bin) continue;
-          bin = (int)((hi - k) >> shift);
-        }
+      each([&](float v, int i) {
+        uint32_t k;
+        if (!held(v, i, &k) || (!start && first_bin >= 0 && bin_of(v) != first_bin)) return;
         const unsigned long long w = f(v, k);
-        if (w) atomicAdd(&hist[bin], w);
-      }
+        if (w) atomicAdd(&hist[start ? bin_of(v) : (int)((hi - k) >> shift)], w);
+      });
       cluster.sync();
       constexpr int kPer = kBins / kThreads;
       unsigned long long mine[kPer], sum = 0;
@@ -302,14 +366,12 @@ struct Row {
         if (w < warp) before += sh.warp_value[w];
         total += sh.warp_value[w];
       }
-      if (share < 0.0 && total < target) return 0;  // every CTA of the row sees the same
-      if (share >= 0.0) {  // the target is a share of the whole, known after the first pass
+      if (share >= 0.0) {  // known after the first pass
         target = (unsigned long long)ceil(__dmul_rn(share, (double)total));
-        if (target < 1) target = 1;
-        if (target > total) target = total;
-        *whole = total;
+        target = target < 1 ? 1 : target > total ? total : target;
         share = -1.0;
       }
+      if (total < target) return;  // every CTA of the row sees the same
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         if (before < target && target <= before + mine[j]) {
@@ -322,7 +384,7 @@ struct Row {
       __syncthreads();
       const int bin = (int)sh.found[0];
       over = sh.found[1];
-      *ties = sh.found[2];
+      ties = sh.found[2];
       __syncthreads();
       if (start) {
         first_bin = bin;
@@ -331,6 +393,8 @@ struct Row {
         const float to = __fsub_rn(top, __fdiv_rn((float)bin + 1.01f, step));
         if (bin > 0) hi = min(hi, key_of(__fadd_rn(from, 0.0f)));
         if (bin < kBins - 1) lo = max(lo, key_of(__fadd_rn(to, 0.0f)));
+        if (sort_border(cut, f, [&](float& v, int i, uint32_t* k) { return held(v, i, k) && bin_of(v) == bin; }, over, target))
+          return;
       } else {
         hi -= (uint32_t)bin << shift;
         const uint32_t width = (1u << shift) - 1;
@@ -338,40 +402,152 @@ struct Row {
         if (shift == 0) break;
       }
     }
-    *above = over;
-    return hi;
+    const unsigned long long w = f(value_of(hi), hi), kept = (target - over + w - 1) / w;
+    cut->last = kept * w < ties ? nth_tie(in, hi, kept) : hi == in.key ? in.last : INT32_MAX;
+    cut->key = hi;
+  }
+
+  // The border among the tokens of one bin, by sorting them in CTA 0; false
+  // when they are more than its list takes.
+  template <typename F, typename H>
+  __device__ bool sort_border(Cut* cut, F f, H in_bin, unsigned long long over, unsigned long long target) {
+    if (tid == 0) sh.listed = 0;
+    cluster.sync();  // also: every CTA has read the histogram that the list replaces
+    Shared* home = cluster.map_shared_rank(&sh, 0);
+    each([&](float v, int i) {
+      uint32_t k;
+      if (!in_bin(v, i, &k) || !f(v, k)) return;
+      const uint32_t slot = atomicAdd(&home->listed, 1u);
+      if (slot < kList) home->list[slot] = (unsigned long long)k << 32 | (kFull - (uint32_t)(base + i));
+    });
+    cluster.sync();
+    unsigned long long found = 0;
+    if (rank == 0 && sh.listed <= kList) {
+      const int n = (int)sh.listed;
+      int n2 = 64;
+      while (n2 < n) n2 <<= 1;
+      for (int i = n + tid; i < n2; i += kThreads) sh.list[i] = 0;
+      __syncthreads();
+      sort_list(sh.list, n2, tid);
+      constexpr int kEach = kList / kThreads;
+      unsigned long long weight[kEach], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const int i = tid * kEach + j;
+        const uint32_t k = i < n ? (uint32_t)(sh.list[i] >> 32) : 0u;
+        weight[j] = i < n ? f(value_of(k), k) : 0ull;
+        sum += weight[j];
+      }
+      const unsigned long long inc = warp_prefix(sum, lane);
+      __syncthreads();
+      if (tid == 0) sh.found[0] = 0;
+      if (lane == 31) sh.warp_value[warp] = inc;
+      __syncthreads();
+      unsigned long long run = over + inc - sum;
+      for (int w = 0; w < warp; ++w) run += sh.warp_value[w];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (run < target && target <= run + weight[j]) sh.found[0] = sh.list[tid * kEach + j];
+        run += weight[j];
+      }
+      __syncthreads();
+      found = sh.found[0];
+    }
+    publish(found, 0, 0);
+    found = peer(0, 0);
+    if (!found) return false;
+    cut->key = (uint32_t)(found >> 32);
+    cut->last = (int)(kFull - (uint32_t)found);
+    return true;
   }
 
   // ---- the first id, ascending, at which a running sum exceeds a target ----
   // One warp's part of f over its segment.
   template <typename F>
-  __device__ __forceinline__ unsigned long long segment_sum(F f) {
+  __device__ __forceinline__ unsigned long long segment_sum(F f) const {
     unsigned long long s = 0;
-    const int begin = warp * p.segment, end = min(n, begin + p.segment);
-#pragma unroll 4
-    for (int i = begin + lane; i < end; i += 32) {
-      const float v = at(i);
+    each([&](float v, int i) {
+      v = v == v ? __fadd_rn(v, 0.0f) : -INFINITY;
       s += f(v, key_of(v), base + i);
-    }
+    });
     return warp_sum(s);
   }
-  // The id for a target in [before, before + the warp's sum); -1 elsewhere.
-  template <typename F>
-  __device__ int locate(F f, unsigned long long before, unsigned long long sum, unsigned long long target) {
-    if (target < before || target >= before + sum) return -1;
-    const int begin = warp * p.segment, end = min(n, begin + p.segment);
-    for (int i = begin; i < end; i += 32) {
-      unsigned long long w = 0;
-      if (i + lane < end) {
-        const float v = at(i + lane);
-        w = f(v, key_of(v), base + i + lane);
-      }
-      const unsigned long long inc = before + warp_prefix(w, lane);
-      const uint32_t past = __ballot_sync(kFull, inc > target);
-      if (past) return base + i + __ffs(past) - 1;
-      before = __shfl_sync(kFull, inc, 31);
+  // The id for a target, from the sums of f before and after each warp's
+  // segment (one warp's `after` is the next one's `before`, to the bit); -1 in the CTAs that do not hold it.  The warp that does
+  // shares its segment out over the block, and then each warp's part is short.
+  // Sums in double may come out a little different there: a target past the
+  // last part's sum is the last id with a weight.
+  template <typename V, typename F>
+  __device__ int locate(F f, V before, V after, V target) {
+    auto bits = [](V v) { unsigned long long b; memcpy(&b, &v, 8); return b; };
+    auto from_bits = [](unsigned long long b) { V v; memcpy(&v, &b, 8); return v; };
+    __syncthreads();
+    if (tid == 0) sh.found[0] = kWarps;
+    __syncthreads();
+    if (lane == 0 && before <= target && target < after) {
+      sh.found[0] = warp;
+      sh.found[1] = bits(before);
     }
-    return -1;
+    __syncthreads();
+    const int owner = (int)sh.found[0];
+    if (owner == kWarps) return -1;  // the whole block
+    before = from_bits(sh.found[1]);
+    int lo = owner * p.segment, hi = min(n, lo + p.segment);
+    constexpr int kFew = 16;  // loads that one warp has in flight at the end
+    while (hi - lo > 32 * kFew) {
+      const int part = ((hi - lo) / 32 + kWarps - 1) / kWarps * 32 + 32;
+      const int begin = min(hi, lo + warp * part), stop = min(hi, begin + part);
+      V sum = 0;
+#pragma unroll 4
+      for (int i = begin + lane; i < stop; i += 32) {
+        const float v = at(i);
+        sum += f(v, key_of(v), base + i);
+      }
+      sum = warp_sum(sum);
+      __syncthreads();
+      if (lane == 0) sh.warp_value[warp] = bits(sum);
+      __syncthreads();
+      V run = before, start = before;
+      int mine = 0;  // the first part whose sum passes the target, or the last with any
+      bool hit = false;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const V s = from_bits(sh.warp_value[w]);
+        if (s > 0 && !hit) {
+          mine = w;
+          start = run;
+          hit = target < run + s;
+        }
+        run += s;
+      }
+      before = start;
+      lo = min(hi, lo + mine * part);
+      hi = min(hi, lo + part);
+    }
+    if (warp == 0) {
+      float v[kFew];
+#pragma unroll
+      for (int k = 0; k < kFew; ++k) v[k] = lo + 32 * k + lane < hi ? at(lo + 32 * k + lane) : -INFINITY;
+      int id = -1;
+      bool hit = false;
+#pragma unroll
+      for (int k = 0; k < kFew; ++k) {
+        const int i = lo + 32 * k;
+        if (hit || i >= hi) continue;
+        const V w = i + lane < hi ? f(v[k], key_of(v[k]), base + i + lane) : V(0);
+        const V inc = before + warp_prefix(w, lane);
+        const uint32_t past = __ballot_sync(kFull, w > 0 && inc > target), some = __ballot_sync(kFull, w > 0);
+        if (some) id = base + i + 31 - __clz(some);
+        if (past) {
+          id = base + i + __ffs(past) - 1;
+          hit = true;
+        }
+        before = __shfl_sync(kFull, inc, 31);
+      }
+      if (lane == 0) sh.found[2] = (unsigned long long)id;
+    }
+    __syncthreads();
+    return (int)sh.found[2];
   }
   // Sums of f before this warp, and of the whole row.
   __device__ __forceinline__ unsigned long long prefix(unsigned long long sum, unsigned long long* total) {
@@ -399,9 +575,8 @@ struct Row {
     const unsigned long long sum = segment_sum(one);
     unsigned long long total;
     const unsigned long long before = prefix(sum, &total);
-    const int id = locate(one, before, sum, count - 1);
-    const unsigned long long mine = block<true>(id >= 0 ? (unsigned long long)id + 1 : 0ull);
-    publish(mine, 0, 0);
+    const int id = locate<unsigned long long>(one, before, before + sum, count - 1);
+    publish((unsigned long long)(id + 1), 0, 0);
     unsigned long long best = 0;
     for (int r = 0; r < ranks; ++r) {
       const unsigned long long o = peer(r, 0);
@@ -411,32 +586,11 @@ struct Row {
   }
 };
 
-// Sorts list[0, 2^m) in descending order (bitonic).
-__device__ void sort_list(unsigned long long* list, int n2, int tid) {
-  for (int size = 2; size <= n2; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      for (int i = tid; i < n2 / 2; i += kThreads) {
-        const int a = 2 * i - (i & (step - 1)), b = a + step;
-        const unsigned long long u = list[a], v = list[b];
-        if ((u < v) == ((a & size) == 0)) {
-          list[a] = v;
-          list[b] = u;
-        }
-      }
-      // pairs up to 32 apart stay within one warp's 64 elements
-      if (step > 32 || (step == 1 && size >= 64))
-        __syncthreads();
-      else
-        __syncwarp();
-    }
-  __syncthreads();
-}
-
 // Puts list[0, n) in the row's order.  The candidates arrived bin by bin, so
 // each takes its place among its bin's; a crowded bin makes that cost more
 // than sorting them all.
 template <int THREADS, typename F>
-__device__ void order_list(Shared& sh, int n, uint32_t at0, bool crowded, int tid, F bin_of_key) {
+__device__ void order_list(Shared& sh, int n, bool crowded, int tid, F bin_of_key) {
   if (crowded) {
     int n2 = 64;
     while (n2 < n) n2 <<= 1;
@@ -451,20 +605,19 @@ __device__ void order_list(Shared& sh, int n, uint32_t at0, bool crowded, int ti
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     const int i = tid + j * THREADS;
-    if (i >= n) break;
+    own[j] = 0;
+    if (i >= n) continue;
     own[j] = sh.list[i];
     const uint32_t bin = bin_of_key((uint32_t)(own[j] >> 32));
-    const uint32_t from = sh.starts[bin] - at0, to = sh.starts[bin + 1] - at0;
+    const uint32_t from = sh.starts[bin], to = sh.starts[bin + 1];
     uint32_t ahead = 0;
     for (uint32_t k = from; k < to; ++k) ahead += sh.list[k] > own[j];
     place[j] = from + ahead;
   }
   if (THREADS == 32) __syncwarp(); else __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    if (tid + j * THREADS >= n) break;
-    sh.list[place[j]] = own[j];
-  }
+  for (int j = 0; j < kEach; ++j)
+    if (own[j]) sh.list[place[j]] = own[j];
   if (THREADS == 32) __syncwarp(); else __syncthreads();
 }
 
@@ -472,19 +625,17 @@ struct Cuts {
   bool by_k, by_p;
   int top_k;
   double top_p, floor_w, u;
-  unsigned long long whole, ahead;  // weights of the row, and before the list
-  bool border_only;                 // the list is about top_p's border: find that
+  unsigned long long whole;  // weights of the row
 };
 
 // The cuts and the draw from the ordered list, by one warp or by the block.
-// Returns 1 when the token is drawn, 0 when the list does not reach top_p's
-// border, or the last candidate that top_p keeps (border_only).
 template <typename T, bool WARP>
-__device__ unsigned long long finish_list(Row<T>& r, const Weigher& weigh, const Cuts& q, int listed) {
+__device__ void finish_list(Row<T>& r, const Weigher& weigh, const Cuts& q, int listed) {
   Shared& sh = r.sh;
   constexpr int kEach = (WARP ? kWarpList : kList) / (WARP ? 32 : kThreads);
   const int tid = r.tid, lane = r.lane, first = tid * kEach;
   auto total_of = [&](unsigned long long v) { return WARP ? warp_sum(v) : r.template block<false>(v); };
+  auto count_of = [&](uint32_t v) { return WARP ? __reduce_add_sync(kFull, v) : (uint32_t)r.template block<false>(v); };
   // thread i holds the ordered candidates kEach i .. kEach i + kEach - 1
   const int in_a = q.by_k ? min(listed, q.top_k) : listed;
   unsigned long long weight[kEach], sum = 0;
@@ -518,8 +669,6 @@ __device__ unsigned long long finish_list(Row<T>& r, const Weigher& weigh, const
     const unsigned long long mass_a = q.by_k ? all : q.whole;
     unsigned long long border = (unsigned long long)ceil(__dmul_rn(q.top_p, (double)mass_a));
     border = border < 1 ? 1 : border > mass_a ? mass_a : border;
-    if (q.ahead >= border || q.ahead + all < border) return 0;
-    border -= q.ahead;
     // those whose running sum before them is below the border
     uint32_t below = 0;
 #pragma unroll
@@ -527,10 +676,9 @@ __device__ unsigned long long finish_list(Row<T>& r, const Weigher& weigh, const
       below += first + j < in_a && run < border;
       run += weight[j];
     }
-    in_c = (int)total_of(below);
-    if (q.border_only) return sh.list[in_c - 1];
+    in_c = (int)count_of(below);
   }
-  in_c = min(in_c, (int)total_of(above_floor));
+  in_c = min(in_c, (int)count_of(above_floor));
   sum = 0;
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
@@ -542,7 +690,36 @@ __device__ unsigned long long finish_list(Row<T>& r, const Weigher& weigh, const
   if (target >= total) target = total - 1;
   uint32_t drawn = 0;
   unsigned long long drawn_weight = 0;
-  if (WARP) {
+  if (WARP && in_c <= 96) {
+    // The candidate whose running sum by id passes target: all pairs.
+    unsigned long long* const weights = sh.list + kWarpList;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (first + j < in_c) weights[first + j] = weight[j];
+    __syncwarp();
+    unsigned long long run[3] = {0, 0, 0}, own[3];
+    uint32_t mark[3];  // smaller ids have larger complements
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      own[j] = lane + 32 * j < in_c ? weights[lane + 32 * j] : 0ull;
+      mark[j] = lane + 32 * j < in_c ? (uint32_t)sh.list[lane + 32 * j] : kFull;
+    }
+#pragma unroll 4
+    for (int k = 0; k < in_c; ++k) {
+      const uint32_t m = (uint32_t)sh.list[k];
+      const unsigned long long w = weights[k];
+#pragma unroll
+      for (int j = 0; j < 3; ++j) run[j] += m > mark[j] ? w : 0ull;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const uint32_t hit = __ballot_sync(kFull, run[j] <= target && target < run[j] + own[j]);
+      if (hit) {
+        drawn = kFull - __shfl_sync(kFull, mark[j], __ffs(hit) - 1);
+        drawn_weight = __shfl_sync(kFull, own[j], __ffs(hit) - 1);
+      }
+    }
+  } else if (WARP) {
     // The lowest id at which the weights up to it exceed target, by halving.
     uint32_t id[kEach];
 #pragma unroll
@@ -563,10 +740,10 @@ __device__ unsigned long long finish_list(Row<T>& r, const Weigher& weigh, const
     for (int j = 0; j < kEach; ++j) drawn_weight += id[j] == drawn ? weight[j] : 0ull;
     drawn_weight = warp_sum(drawn_weight);
   } else {
-    // The same, 256 ranges of ids at a time, by their weights.
+    // The same, a range of ids per thread at a time, by their weights.
     unsigned long long* ranges = reinterpret_cast<unsigned long long*>(sh.counts);
     static_assert(sizeof(sh.counts) >= kThreads * sizeof(unsigned long long), "a range per thread");
-    for (int shift = max(0, 32 - 8 - __clz((uint32_t)r.p.vocab));; shift = max(0, shift - 8)) {
+    for (int shift = max(0, 32 - kThreadBits - __clz((uint32_t)r.p.vocab));; shift = max(0, shift - kThreadBits)) {
       __syncthreads();
       ranges[tid] = 0;
       __syncthreads();
@@ -574,7 +751,7 @@ __device__ unsigned long long finish_list(Row<T>& r, const Weigher& weigh, const
       for (int j = 0; j < kEach; ++j)
         if (weight[j]) {
           const uint32_t id = kFull - (uint32_t)sh.list[first + j], at = (id - drawn) >> shift;
-          if (id >= drawn && at < 256) atomicAdd(&ranges[at], weight[j]);
+          if (id >= drawn && at < kThreads) atomicAdd(&ranges[at], weight[j]);
         }
       __syncthreads();
       const unsigned long long mine = ranges[tid], inc = warp_prefix(mine, lane);
@@ -601,7 +778,82 @@ __device__ unsigned long long finish_list(Row<T>& r, const Weigher& weigh, const
     r.p.tokens[row] = (int32_t)drawn;
     if (r.p.probs) r.p.probs[row] = (float)__ddiv_rn((double)drawn_weight, (double)total);
   }
-  return 1;
+}
+
+// The bins of a row's logits: bin = round(step (reference - v)) + kAhead or so,
+// as the sum of a constant, v times -step and 1.5 * 2^23, whose last bits are
+// the rounded whole number.  It never decreases as v falls; what lies above
+// the bins is in bin 0, NaN and what lies below them in none (kCoarse or more).
+struct Bins {
+  float step, origin, lead, halvings;  // lead: the reference's place; halvings: of the weight, per bin
+  __device__ __forceinline__ uint32_t of(float v) const {
+    return (uint32_t)max((int)(__float_as_uint(__fmaf_rn(v, -step, origin)) - 0x4B400000u), 0);
+  }
+  __device__ __forceinline__ uint32_t of_key(uint32_t key) const { return of(value_of(key)); }
+  // False where a range or reference has no such bins.
+  __device__ __forceinline__ bool set(float reference, float range, double rate) {
+    if (!(range > 0.0f && range < 1e30f && fabsf(reference) < 1e30f)) return false;
+    step = __fdiv_rn((float)(kCoarse - 8), range);
+    if (!(__fmul_rn(fabsf(reference), step) < 4194304.0f)) return false;  // the constant would lose the bins
+    origin = __fadd_rn(__fmul_rn(reference, step), 12582912.0f + (float)kAhead);
+    lead = __fmaf_rn(-reference, step, __fsub_rn(origin, 12582912.0f));
+    halvings = __fdiv_rn((float)rate, step);
+    return true;
+  }
+};
+
+// Where the cuts lie in a histogram of counts, two bins per thread: starts[]
+// are its prefix sums; *last is the first bin that satisfies a cut (kCoarse - 1
+// when none does), *first a bin before top_p's border (or the k-th logit's).
+// `whole`: the sum of all weights, or 0 to take the bins' own estimate; slack:
+// how far beside its share top_p's border is looked for.
+template <typename T>
+__device__ __forceinline__ void find_cuts(Row<T>& r, const Bins& bins, uint32_t c0, uint32_t c1, const Cuts& q, float share,
+                                          float whole, float floor_bin, uint32_t* last, bool* crowded) {
+  Shared& sh = r.sh;
+  const int tid = r.tid, lane = r.lane, bin0 = 2 * tid;
+  static_assert(kCoarse == 2 * kThreads, "a thread has two bins");
+  // Counts and least weights up to each bin, both in one scan.
+  const float w0 = __fmul_rn((float)c0, exp2_approx(__fmul_rn(bins.halvings, __fsub_rn(bins.lead, (float)bin0 + 0.52f))));
+  const float w1 = __fmul_rn((float)c1, exp2_approx(__fmul_rn(bins.halvings, __fsub_rn(bins.lead, (float)bin0 + 1.52f))));
+  uint32_t count = c0 + c1;
+  float mass = __fadd_rn(w0, w1);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t a = __shfl_up_sync(kFull, count, o);
+    const float b = __shfl_up_sync(kFull, mass, o);
+    if (lane >= o) {
+      count += a;
+      mass = __fadd_rn(mass, b);
+    }
+  }
+  __syncthreads();
+  if (lane == 31) sh.warp_value[r.warp] = (unsigned long long)count << 32 | __float_as_uint(mass);
+  if (tid == 0) sh.found[0] = kCoarse;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    const unsigned long long o = sh.warp_value[i];
+    if (i < r.warp) {
+      count += (uint32_t)(o >> 32);
+      mass = __fadd_rn(mass, __uint_as_float((uint32_t)o));
+    }
+  }
+  sh.starts[bin0] = count - c0 - c1;
+  sh.starts[bin0 + 1] = count - c1;
+  if (tid == kThreads - 1) sh.starts[kCoarse] = count;
+  const float past_p = __fmul_rn(__fmul_rn(share, whole), 1.0001f);
+  const bool p_alone = q.by_p && !q.by_k;
+  auto enough = [&](int bin, uint32_t c, float m) {
+    return (q.by_k && c >= (uint32_t)q.top_k) || (p_alone && c > 0 && m >= past_p) || (!q.by_p && c > 0 && (float)bin >= floor_bin);
+  };
+  if (enough(bin0, count - c1, __fsub_rn(mass, w1)))
+    atomicMin(&sh.found[0], (unsigned long long)bin0);
+  else if (enough(bin0 + 1, count, mass))
+    atomicMin(&sh.found[0], (unsigned long long)(bin0 + 1));
+  __syncthreads();
+  *last = (uint32_t)sh.found[0];
+  *crowded = __syncthreads_or((bin0 <= (int)*last && c0 > kCrowd) || (bin0 + 1 <= (int)*last && c1 > kCrowd));
 }
 
 template <typename T>
@@ -615,6 +867,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   const int slice = p.segment * kWarps, base = min(p.vocab, rank * slice), n = min(slice, p.vocab - base);
   if (tid < 64) sh.powers[tid] = exp2(-(double)tid / 64.0);
   for (int i = tid; i < kCoarse; i += kThreads) sh.counts[i] = sh.filled[i] = 0;
+  if (tid == 0) sh.listed = 0;
   pdl_enter();
 
   // ---- the logits, once ----
@@ -626,12 +879,12 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
                  : "memory");
 #pragma unroll 8
   for (int i = vecs * kVec + tid; i < n; i += kThreads) x[i] = src[i];
+  for (int i = n + tid; i < (n + kVec - 1) / kVec * kVec; i += kThreads) x[i] = Logit<T>::none();
   const float temperature = p.temperature ? p.temperature[row] : 1.0f;
   const int top_k = p.top_k ? p.top_k[row] : 0;
   const float top_p = p.top_p ? p.top_p[row] : 1.0f;
   const float min_p = p.min_p ? p.min_p[row] : 0.0f;
   const double u = fmin(fmax((double)p.uniform[row], 0.0), 1.0);
-  for (int i = n + tid; i < (n + kVec - 1) / kVec * kVec; i += kThreads) x[i] = Logit<T>::none();
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
   if (p.candidates) {
@@ -640,40 +893,23 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       if (!(mask[(base + i) >> 5] >> ((base + i) & 31) & 1)) x[i] = Logit<T>::none();
     __syncthreads();
   }
-  // One pass over the slice, 16 bytes at a time: f(logit, id).
-  const int all_vecs = (n + kVec - 1) / kVec;
-  auto each = [&](auto f) {
-    for (int i = tid; i < all_vecs; i += kThreads) {
-      const uint4 q = *reinterpret_cast<const uint4*>(x + i * kVec);
-      T t[kVec];
-      memcpy(t, &q, 16);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) f(Logit<T>::get(t[j]), i * kVec + j);
-    }
-  };
+  Row<T> r{p, sh, x, cluster, ranks, rank, base, n, tid, lane, tid >> 5, 0, 0};
   float most = -INFINITY, least = INFINITY;
   bool nan = false;
-  each([&](float v, int) {
+  r.each([&](float v, int) {
     most = fmaxf(most, v);
     least = fminf(least, v);
     nan |= v != v;
   });
   if (nan) flag_status(p.status, kStatusNonFinite);
-
-  Row<T> r{p, sh, x, cluster, ranks, rank, base, n, tid, lane, tid >> 5, 0, 0};
-  {
-    uint32_t a = key_of(most), b = ~key_of(least);
-    r.block_max2(a, b);
-    r.publish(a, b, 0);
-  }
-  unsigned long long top_bits = 0, least_bits = 0;
+  uint32_t key_max = key_of(__fadd_rn(most, 0.0f)), key_low = ~key_of(least);
+  r.block_max2(key_max, key_low);
+  r.publish(key_max, key_low, 0);
   for (int i = 0; i < ranks; ++i) {
-    const unsigned long long a = r.peer(i, 0), b = r.peer(i, 1);
-    top_bits = a > top_bits ? a : top_bits;
-    least_bits = b > least_bits ? b : least_bits;
+    key_max = max(key_max, (uint32_t)r.peer(i, 0));
+    key_low = max(key_low, (uint32_t)r.peer(i, 1));
   }
-  const float top = __fadd_rn(value_of((uint32_t)top_bits), 0.0f);  // -0 is 0
-  const uint32_t key_max = key_of(top);
+  const float top = value_of(key_max);
   const bool refused = !(temperature >= 0.0f);
   if (refused || top == -INFINITY) {
     if (rank == 0 && tid == 0) {
@@ -686,200 +922,104 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   }
   if (temperature == 0.0f) {
     uint32_t id = kFull;
-    each([&](float v, int i) {
+    r.each([&](float v, int i) {
       if (v == top) id = min(id, (uint32_t)(base + i));
     });
-    r.publish(r.template block<true>((unsigned long long)(kFull - id)), 0, 0);
+    uint32_t inverse = kFull - id, none = 0;
+    r.block_max2(inverse, none);
+    r.publish(inverse, 0, 0);
     if (rank == 0 && tid == 0) {
-      unsigned long long best = 0;
-      for (int i = 0; i < ranks; ++i) {
-        const unsigned long long o = r.peer(i, 0);
-        best = o > best ? o : best;
-      }
-      p.tokens[row] = (int32_t)(kFull - (uint32_t)best);
+      for (int i = 0; i < ranks; ++i) inverse = max(inverse, (uint32_t)r.peer(i, 0));
+      p.tokens[row] = (int32_t)(kFull - inverse);
       if (p.probs) p.probs[row] = 1.0f;
     }
     cluster.sync();
     return;
   }
-  const Weigher weigh{(double)top, __ddiv_rn(1.4426950408889634074, (double)temperature), key_max, sh.powers};
-  const double floor_w = min_p > 0.0f ? fmin((double)min_p, 1.0) : 0.0;
-  const float low = value_of(~(uint32_t)least_bits);
-  const float range = fminf(__fmul_rn(kReach, temperature), __fsub_rn(top, low));
-  const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0f;
+  const Weigher weigh(top, (double)temperature, sh.powers);
+  const float reach = __fmul_rn(kReach, temperature), lowest = __fsub_rn(top, reach);  // below it weights vanish
+  const bool regular = __dmul_rn(fabs((double)top), weigh.rate) < 4398046511104.0;  // 2^42: near() holds
+  const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0f, by_floor = min_p > 0.0f;
+  const double floor_p = by_floor ? fmin((double)min_p, 1.0) : 0.0;
+  const float share = fmaxf(top_p, 0.0f);
 
   // ---- the few that matter, in one CTA ----
-  Cut cut{kKeyNone, -1};
-  bool cut_found = false;
-  if ((by_k || by_p || floor_w > 0.0) && range > 0.0f && range < 1e30f && top < INFINITY) {
-    // bin = round(step (top - v) + 2 or so): the sum of a constant, v times
-    // -step and 1.5 * 2^23, whose last bits are the rounded whole number; it
-    // never decreases as v falls.  NaN and what lies out of reach end above kCoarse.
-    const float step = __fdiv_rn((float)(kCoarse - 8), range);
-    const float origin = __fadd_rn(__fmul_rn(top, step), 12582912.0f + 2.0f);
-    if (__fmul_rn(fabsf(top), step) < 4194304.0f) {  // else the constant loses the bins
-      const float lead = __fmaf_rn(-top, step, __fsub_rn(origin, 12582912.0f));  // the top's place, about 2
-      auto bin_of = [&](float v) { return __float_as_uint(__fmaf_rn(v, -step, origin)) - 0x4B400000u; };
-      const bool need_whole = by_p && !by_k;
-      unsigned long long whole = 0;
-      if (need_whole) {
-        each([&](float v, int) {
-          const uint32_t b = bin_of(v);
-          const unsigned long long w = Weigher::fixed(weigh.near(v));
-          if (b < kCoarse) {
-            atomicAdd(&sh.counts[b], 1u);
-            whole += w;
-          }
-        });
-        whole = r.template block<false>(whole);
-      } else {
-        each([&](float v, int) {
-          const uint32_t b = bin_of(v);
-          if (b < kCoarse) atomicAdd(&sh.counts[b], 1u);
-        });
-      }
-      __syncthreads();
-      r.publish(whole, 0, 0);
-      static_assert(kCoarse == 2 * kThreads, "a thread has two bins");
-      uint32_t c0 = 0, c1 = 0;
-      whole = 0;
-      for (int i = 0; i < ranks; ++i) {
-        const uint2 o = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&sh, i)->counts)[tid];
-        c0 += o.x;
-        c1 += o.y;
-        whole += r.peer(i, 0);
-      }
-      // Counts and estimated weights up to each bin, both in one scan.
-      const float bits = __fdiv_rn((float)weigh.rate, step);  // halvings per bin
-      const int bin0 = 2 * tid;
-      const float w0 = __fmul_rn((float)c0, exp2_approx(__fmul_rn(bits, __fsub_rn(lead, (float)bin0))));
-      const float w1 = __fmul_rn((float)c1, exp2_approx(__fmul_rn(bits, __fsub_rn(lead, (float)(bin0 + 1)))));
-      uint32_t count = c0 + c1;
-      float mass = __fadd_rn(w0, w1);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t a = __shfl_up_sync(kFull, count, o);
-        const float b = __shfl_up_sync(kFull, mass, o);
-        if (lane >= o) {
-          count += a;
-          mass = __fadd_rn(mass, b);
+  Bins bins;
+  if ((by_k || by_p || by_floor) && regular &&
+      bins.set(top, fminf(reach, __fsub_rn(top, value_of(~key_low))), weigh.rate)) {
+    Cuts q{by_k, by_p, top_k, (double)share, floor_p, u, 0};
+    unsigned long long whole = 0;
+    if (by_p && !by_k) {
+      r.each([&](float v, int) {
+        const uint32_t b = bins.of(v);
+        const unsigned long long w = Weigher::fixed(weigh.near(v));
+        if (b < kCoarse) {
+          atomicAdd(&sh.counts[b], 1u);
+          whole += w;
         }
+      });
+      whole = r.template block<false>(whole);
+    } else {
+      r.each([&](float v, int) {
+        const uint32_t b = bins.of(v);
+        if (b < kCoarse) atomicAdd(&sh.counts[b], 1u);
+      });
+    }
+    __syncthreads();
+    r.publish(whole, 0, 0);
+    uint32_t c0 = 0, c1 = 0;
+    for (int i = 0; i < ranks; ++i) {
+      const uint2 o = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&sh, i)->counts)[tid];
+      c0 += o.x;
+      c1 += o.y;
+      q.whole += r.peer(i, 0);
+    }
+    const float floor_bin = by_floor ? __fadd_rn(__fdiv_rn(-log2f((float)floor_p), bins.halvings), bins.lead + 3.0f) : 1e30f;
+    uint32_t last;
+    bool crowded;
+    find_cuts(r, bins, c0, c1, q, share, __fmul_rn((float)q.whole, 1.0f / 1099511627776.0f), floor_bin, &last, &crowded);
+    const uint32_t listed = last < kCoarse ? sh.starts[last + 1] : kList + 1;
+    if (listed <= kList) {
+      Shared* home = cluster.map_shared_rank(&sh, 0);
+      r.each([&](float v, int i) {
+        const uint32_t b = bins.of(v);
+        if (b > last) return;
+        v = __fadd_rn(v, 0.0f);
+        const uint32_t slot = sh.starts[b] + atomicAdd(&home->filled[b], 1u);
+        if (slot < kList) home->list[slot] = (unsigned long long)key_of(v) << 32 | (kFull - (uint32_t)(base + i));
+      });
+      cluster.sync();
+      // the list holds every cut: the other CTAs, and for short lists the
+      // other warps, are done
+      if (rank != 0) return;
+      auto bin_of_key = [&](uint32_t key) { return bins.of_key(key); };
+      if (listed > kWarpList || crowded) {
+        order_list<kThreads>(sh, (int)listed, crowded, tid, bin_of_key);
+        finish_list<T, false>(r, weigh, q, (int)listed);
+      } else if (tid < 32) {
+        order_list<32>(sh, (int)listed, false, tid, bin_of_key);
+        finish_list<T, true>(r, weigh, q, (int)listed);
       }
-      if (lane == 31) sh.warp_value[tid >> 5] = (unsigned long long)count << 32 | __float_as_uint(mass);
-      if (tid == 0) sh.found[0] = sh.found[1] = kCoarse - 1;
-      __syncthreads();
-      float mass_total = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        const unsigned long long o = sh.warp_value[i];
-        if (i < (tid >> 5)) {
-          count += (uint32_t)(o >> 32);
-          mass = __fadd_rn(mass, __uint_as_float((uint32_t)o));
-        }
-        mass_total = __fadd_rn(mass_total, __uint_as_float((uint32_t)o));
-      }
-      sh.starts[bin0] = count - c0 - c1;
-      sh.starts[bin0 + 1] = count - c1;
-      if (tid == kThreads - 1) sh.starts[kCoarse] = count;
-      // The last bin that can matter: the first that satisfies any of the
-      // cuts.  For a top_p of many tokens also the first bin near its border.
-      const float share = fmaxf(top_p, 0.0f);
-      const float near_p = __fmul_rn(__fsub_rn(share, 0.005f), mass_total), past_p = __fmul_rn(__fadd_rn(share, 0.01f), mass_total);
-      const float floor_bin = floor_w > 0.0 ? __fadd_rn(__fdiv_rn(-log2f((float)floor_w), bits), 6.0f) : 1e30f;
-      auto enough = [&](int bin, uint32_t c, float m) {
-        return (by_k && c >= (uint32_t)top_k) || (need_whole && m >= past_p) || (!by_p && (float)bin >= floor_bin);
-      };
-      if (enough(bin0, count - c1, __fsub_rn(mass, w1)))
-        atomicMin(&sh.found[0], (unsigned long long)bin0);
-      else if (enough(bin0 + 1, count, mass))
-        atomicMin(&sh.found[0], (unsigned long long)(bin0 + 1));
-      if (need_whole && mass >= near_p) atomicMin(&sh.found[1], (unsigned long long)bin0);
-      __syncthreads();
-      const uint32_t last = (uint32_t)sh.found[0];
-      const bool crowded = __syncthreads_or((bin0 <= (int)last && c0 > kCrowd) || (bin0 + 1 <= (int)last && c1 > kCrowd));
-      // All candidates, or, where they are too many, those about top_p's border.
-      uint32_t from = 0;
-      if (sh.starts[last + 1] > kList && need_whole) from = (uint32_t)min(sh.found[1], sh.found[0]);
-      const uint32_t at0 = sh.starts[from], listed = sh.starts[last + 1] - at0;
-      if (listed <= kList) {
-        Shared* home = cluster.map_shared_rank(&sh, 0);
-        unsigned long long ahead = 0;  // the weights before the list
-        each([&](float v, int i) {
-          const uint32_t b = bin_of(v);
-          if (b > last) return;
-          v = __fadd_rn(v, 0.0f);
-          if (b < from) {
-            ahead += Weigher::fixed(weigh.near(v));
-            return;
-          }
-          const uint32_t slot = sh.starts[b] - at0 + atomicAdd(&home->filled[b], 1u);
-          if (slot < kList) home->list[slot] = (unsigned long long)key_of(v) << 32 | (kFull - (uint32_t)(base + i));
-        });
-        if (from) ahead = r.template block<false>(ahead);
-        r.publish(ahead, 0, 0);  // and the list is complete
-        unsigned long long outcome = 0;
-        if (rank == 0 && (listed > kWarpList || crowded || from || tid < 32)) {
-          ahead = 0;
-          if (from)
-            for (int i = 0; i < ranks; ++i) ahead += r.peer(i, 0);
-          const Cuts cuts{by_k, by_p, top_k, fmax((double)top_p, 0.0), floor_w, u, whole, ahead, from > 0};
-          auto value_bin = [&](uint32_t key) { return bin_of(value_of(key)); };
-          if (listed > kWarpList || crowded || from) {
-            order_list<kThreads>(sh, (int)listed, at0, crowded, tid, value_bin);
-            outcome = finish_list<T, false>(r, weigh, cuts, (int)listed);
-          } else {
-            order_list<32>(sh, (int)listed, at0, false, tid, value_bin);
-            outcome = finish_list<T, true>(r, weigh, cuts, (int)listed);
-          }
-        }
-        if (!need_whole) return;  // nothing was estimated: the list held every cut
-        // Every CTA learns whether the list reached top_p's border: 1 = drawn,
-        // more = the cut, for a draw from all.
-        r.publish(outcome, 0, 0);
-        outcome = r.peer(0, 0);
-        if (outcome == 1) {
-          cluster.sync();  // no CTA leaves while another may read its shared memory
-          return;
-        }
-        if (outcome) {
-          cut.key = (uint32_t)(outcome >> 32);
-          cut.last = (int)(kFull - (uint32_t)outcome);
-          cut_found = true;
-        }
-      }
+      return;
     }
   }
 
   // ---- the general way: top-k, then top-p ----
-  const uint32_t key_min = max(kKeyNone + 1, key_of(__fsub_rn(top, __fmul_rn(kReach, temperature))));
-  unsigned long long above, ties, whole;
-  if (by_k) {
-    auto one = [](float, uint32_t) -> unsigned long long { return 1; };
-    const uint32_t key = r.border(cut, one, top_k, top, range, key_min, key_max, &above, &ties, &whole, -1.0);
-    if (key) {
-      const unsigned long long kept = (unsigned long long)top_k - above;
-      cut.last = kept < ties ? r.nth_tie(cut, key, kept) : INT32_MAX;
-      cut.key = key;
-    }
-  }
-  if (by_p && !cut_found) {
-    auto mass = [&](float v, uint32_t k) { return Weigher::fixed(weigh.real(v, k)); };
-    const uint32_t key = r.border(cut, mass, 0, top, range, max(key_min, cut.key), key_max, &above, &ties, &whole,
-                                  fmax((double)top_p, 0.0));
-    unsigned long long target = (unsigned long long)ceil(__dmul_rn(fmax((double)top_p, 0.0), (double)whole));
-    target = target < 1 ? 1 : target > whole ? whole : target;
-    const unsigned long long w = mass(value_of(key), key);
-    const unsigned long long kept = (target - above + w - 1) / w;
-    const int last = kept * w < ties ? r.nth_tie(cut, key, kept) : (key == cut.key ? cut.last : INT32_MAX);
-    cut.key = key;
-    cut.last = last;
-  }
+  const uint32_t key_min = max(kKeyNone + 1, key_of(__fsub_rn(top, reach)));
+  auto fixed_weight = [&](float v, uint32_t k) -> unsigned long long {
+    if (!regular) return Weigher::fixed(weigh.real(v, k));
+    const unsigned long long w = Weigher::fixed(weigh.near(v));
+    return v >= lowest ? w : 0ull;
+  };
+  Cut cut{kKeyNone, -1};
+  if (by_k) r.border(&cut, [](float, uint32_t) { return 1ull; }, top_k, top, reach, key_min, key_max, -1.0);
+  if (by_p) r.border(&cut, fixed_weight, 0, top, reach, max(key_min, cut.key), key_max, (double)share);
 
-  // ---- the draw ----
+  // ---- the draw from all ----
   auto weight = [&](float v, uint32_t k, int id) -> unsigned long long {
     if (!cut.holds(k, id)) return 0;
-    const double w = weigh.real(v, k);
-    return w >= floor_w ? Weigher::fixed(w) : 0ull;
+    if (by_floor && !(weigh.real(v, k) >= floor_p)) return 0;
+    return fixed_weight(v, k);
   };
   const unsigned long long sum = r.segment_sum(weight);
   unsigned long long total;
@@ -887,8 +1027,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // running > u * total  <=>  running > floor(u * total) for whole numbers
   unsigned long long target = (unsigned long long)floor(__dmul_rn(u, (double)total));
   if (target >= total) target = total - 1;
-  const int id = r.locate(weight, before, sum, target);
-  if (id >= 0 && lane == 0) {
+  const int id = r.template locate<unsigned long long>(weight, before, before + sum, target);
+  if (id >= 0 && tid == 0) {
     p.tokens[row] = id;
     const float v = r.at(id - base);
     if (p.probs) p.probs[row] = (float)__ddiv_rn((double)weight(v, key_of(v), id), (double)total);
