@@ -6,24 +6,13 @@
 // keys with the running maximum and sum of each row in registers.
 #include <cstring>
 
-#include "decode_ops.cuh"
+#include "cross_attn.cuh"
 
 namespace mc {
 namespace {
 
 constexpr uint32_t kFull = 0xFFFFFFFFu;
 constexpr int kSms = 148;
-
-struct CrossParams {
-  AttnRows rows;
-  AttnSplit split;
-  const void *k, *v;
-  long long k_rs, k_hs, v_rs, v_hs;
-  const uint8_t* mask;
-  float scale;
-  int row_tiles;
-  uint32_t* status;
-};
 
 // ---- small tiles: mma.sync ------------------------------------------------------------
 // Four warps: WR of them side by side over 16 rows each, the other 4 / WR
@@ -450,36 +439,47 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
 
 // ---- shapes of a launch ----
 struct CrossPlan {
-  int warps_rows, row_tiles, splits, chunk, tile_keys;
+  bool long_tiles;
+  int tile_rows, row_tiles, splits, chunk, tile_keys;
   long long units;
   uint64_t slots, bytes;
 };
 
-bool cross_plan(const mc_cross_attention_args* a, CrossPlan* plan) {
-  if (!a || dtype_bytes(a->dtype) == 0 || a->batch < 0 || a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads != 0 ||
-      a->head_dim < 16 || a->head_dim > kOpMaxHeadDim || a->head_dim % 16 != 0 || a->max_q_len < 0 || a->max_k_len < 0 ||
-      a->heads > 65536)
-    return false;
+bool cross_sizes_ok(const mc_cross_attention_args* a) {
+  return a && dtype_bytes(a->dtype) != 0 && a->batch >= 0 && a->kv_heads >= 1 && a->heads >= 1 &&
+         a->heads % a->kv_heads == 0 && a->head_dim >= 16 && a->head_dim <= kOpMaxHeadDim && a->head_dim % 16 == 0 &&
+         a->max_q_len >= 0 && a->max_k_len >= 0 && a->heads <= 65536 &&
+         (int64_t)(a->heads / a->kv_heads) * a->max_q_len <= INT32_MAX / 2 &&
+         (int64_t)a->batch * a->kv_heads * ((int64_t)(a->heads / a->kv_heads) * a->max_q_len / 16 + 1) <= INT32_MAX;
+}
+
+// Long tiles pay where a sequence's rows fill most of two of them and its keys
+// a few: below, the small kernel's 16-row warps waste less.
+bool long_pays(const mc_cross_attention_args* a) {
+  return a->dtype != MC_F32 && !a->key_mask && a->scale > 0.0f && cross_long_strides(a) &&
+         (int64_t)(a->heads / a->kv_heads) * a->max_q_len >= 128 && a->max_k_len >= 128;
+}
+
+CrossPlan cross_plan(const mc_cross_attention_args* a, bool long_tiles) {
+  CrossPlan plan;
   const int64_t rows = (int64_t)(a->heads / a->kv_heads) * a->max_q_len;
-  if (rows > INT32_MAX / 2) return false;
-  plan->tile_keys = a->dtype == MC_F32 ? 32 : 64;
-  plan->warps_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int tile_rows = 16 * plan->warps_rows;
-  plan->row_tiles = (int)((rows + tile_rows - 1) / tile_rows);
-  plan->units = (int64_t)a->batch * a->kv_heads * plan->row_tiles;
-  if (plan->units > INT32_MAX) return false;
-  // Ranges of keys for units too few to fill the GPU (three CTAs per SM),
-  // each of four tiles at least.
-  const int tiles = (int)(((int64_t)a->max_k_len + plan->tile_keys - 1) / plan->tile_keys);
-  long long splits = plan->units > 0 ? kSms * 3 / plan->units : 1;
+  plan.long_tiles = long_tiles;
+  plan.tile_keys = long_tiles ? kLongKeys : a->dtype == MC_F32 ? 32 : 64;
+  plan.tile_rows = long_tiles ? kLongRows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  plan.row_tiles = (int)((rows + plan.tile_rows - 1) / plan.tile_rows);
+  plan.units = (int64_t)a->batch * a->kv_heads * plan.row_tiles;
+  // Ranges of keys for units too few to fill the GPU (one long CTA or three
+  // small ones per SM), each of four tiles at least.
+  const int tiles = (int)(((int64_t)a->max_k_len + plan.tile_keys - 1) / plan.tile_keys);
+  long long splits = plan.units > 0 ? kSms * (long_tiles ? 1 : 3) / plan.units : 1;
   if (splits > tiles / 4) splits = tiles / 4;
   if (splits > 256) splits = 256;
   if (splits < 1) splits = 1;
-  plan->chunk = tiles > 0 ? (int)((tiles + splits - 1) / splits) : 1;
-  plan->splits = tiles > 0 ? (tiles + plan->chunk - 1) / plan->chunk : 1;
-  plan->slots = (uint64_t)plan->units * tile_rows;
-  plan->bytes = attn_split_bytes(plan->slots, plan->splits, a->head_dim);
-  return true;
+  plan.chunk = tiles > 0 ? (int)((tiles + splits - 1) / splits) : 1;
+  plan.splits = tiles > 0 ? (tiles + plan.chunk - 1) / plan.chunk : 1;
+  plan.slots = (uint64_t)plan.units * plan.tile_rows;
+  plan.bytes = attn_split_bytes(plan.slots, plan.splits, a->head_dim);
+  return plan;
 }
 
 template <typename T, int D, int WR>
@@ -493,8 +493,8 @@ cudaError_t launch_small(const CrossParams& p, const CrossPlan& plan, cudaStream
 
 template <typename T, int D>
 cudaError_t launch_small_w(const CrossParams& p, const CrossPlan& plan, cudaStream_t s) {
-  return plan.warps_rows == 1   ? launch_small<T, D, 1>(p, plan, s)
-         : plan.warps_rows == 2 ? launch_small<T, D, 2>(p, plan, s)
+  return plan.tile_rows == 16   ? launch_small<T, D, 1>(p, plan, s)
+         : plan.tile_rows == 32 ? launch_small<T, D, 2>(p, plan, s)
                                 : launch_small<T, D, 4>(p, plan, s);
 }
 
@@ -505,20 +505,49 @@ cudaError_t launch_small_t(const CrossParams& p, const CrossPlan& plan, cudaStre
                                   : launch_small_w<__nv_bfloat16, D>(p, plan, s);
 }
 
+cudaError_t launch_small_d(const CrossParams& p, const CrossPlan& plan, cudaStream_t s) {
+  switch (p.rows.head_dim) {
+    case 16: return launch_small_t<16>(p, plan, s);
+    case 32: return launch_small_t<32>(p, plan, s);
+    case 48: return launch_small_t<48>(p, plan, s);
+    case 64: return launch_small_t<64>(p, plan, s);
+    case 80: return launch_small_t<80>(p, plan, s);
+    case 96: return launch_small_t<96>(p, plan, s);
+    case 112: return launch_small_t<112>(p, plan, s);
+    case 128: return launch_small_t<128>(p, plan, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_cross(CrossParams p, const CrossPlan& plan, void* workspace, cudaStream_t s) {
+  p.split.splits = plan.splits;
+  p.split.chunk = plan.chunk;
+  p.row_tiles = plan.row_tiles;
+  if (plan.splits > 1) {
+    p.split.out = static_cast<float*>(workspace);
+    p.split.lse = p.split.out + plan.slots * plan.splits * p.rows.head_dim;
+  }
+  const cudaError_t e = plan.long_tiles ? launch_cross_long(p, plan.units, s) : launch_small_d(p, plan, s);
+  if (e != cudaSuccess || plan.splits <= 1) return e;
+  return launch_attn_join(p.rows, p.split, plan.tile_keys, plan.tile_rows, plan.row_tiles, s);
+}
+
 }  // namespace
 }  // namespace mc
 
 extern "C" uint64_t mc_cross_attention_workspace(const mc_cross_attention_args* args) {
-  mc::CrossPlan plan;
-  return mc::cross_plan(args, &plan) ? plan.bytes : 0;
+  if (!mc::cross_sizes_ok(args)) return 0;
+  // either kernel may run: which one also goes by the strides and the mask
+  const uint64_t small = mc::cross_plan(args, false).bytes;
+  const uint64_t wide = args->dtype == MC_F32 ? 0 : mc::cross_plan(args, true).bytes;
+  return small > wide ? small : wide;
 }
 
 extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* stream) {
-  mc::CrossPlan plan;
-  if (!mc::cross_plan(a, &plan) || !isfinite(a->scale) || a->q_rows < 0 || a->q_rows > INT32_MAX || a->k_rows < 0 ||
+  if (!mc::cross_sizes_ok(a) || !isfinite(a->scale) || a->q_rows < 0 || a->q_rows > INT32_MAX || a->k_rows < 0 ||
       a->k_rows > INT32_MAX)
     return MC_INVALID_INPUT;
-  if (plan.units == 0) return MC_OK;
+  if (a->batch == 0 || a->max_q_len == 0) return MC_OK;
   const int bytes = mc::dtype_bytes(a->dtype);
   if (!a->q_start || !a->q_len || !a->k_start || !a->k_len || !mc::aligned4(a->q_start) || !mc::aligned4(a->q_len) ||
       !mc::aligned4(a->k_start) || !mc::aligned4(a->k_len) || !mc::aligned4(a->lse) ||
@@ -529,8 +558,8 @@ extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* 
       !mc::strides_apart(a->q_rows, a->heads, a->head_dim, a->out_row_stride, a->out_head_stride) || a->out == a->q ||
       a->out == a->k || a->out == a->v)
     return MC_INVALID_INPUT;
-  if (plan.bytes > 0 && (!a->workspace || !mc::aligned16(a->workspace) || a->workspace_bytes < plan.bytes))
-    return MC_INVALID_INPUT;
+  const uint64_t need = mc_cross_attention_workspace(a);
+  if (need > 0 && (!a->workspace || !mc::aligned16(a->workspace) || a->workspace_bytes < need)) return MC_INVALID_INPUT;
   mc_status where = mc::on_current_device(a->q);
   if (where == MC_OK) where = mc::on_current_device(a->k);
   if (where != MC_OK) return where;
@@ -559,12 +588,6 @@ extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* 
   r.head_dim = a->head_dim;
   r.max_q = a->max_q_len;
   r.max_k = a->max_k_len;
-  p.split.splits = plan.splits;
-  p.split.chunk = plan.chunk;
-  if (plan.splits > 1) {
-    p.split.out = static_cast<float*>(a->workspace);
-    p.split.lse = p.split.out + plan.slots * plan.splits * a->head_dim;
-  }
   p.k = a->k;
   p.v = a->v;
   p.k_rs = a->k_row_stride;
@@ -573,22 +596,10 @@ extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* 
   p.v_hs = a->v_head_stride;
   p.mask = a->key_mask;
   p.scale = a->scale;
-  p.row_tiles = plan.row_tiles;
   p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaErrorInvalidValue;
-  switch (a->head_dim) {
-    case 16: e = mc::launch_small_t<16>(p, plan, s); break;
-    case 32: e = mc::launch_small_t<32>(p, plan, s); break;
-    case 48: e = mc::launch_small_t<48>(p, plan, s); break;
-    case 64: e = mc::launch_small_t<64>(p, plan, s); break;
-    case 80: e = mc::launch_small_t<80>(p, plan, s); break;
-    case 96: e = mc::launch_small_t<96>(p, plan, s); break;
-    case 112: e = mc::launch_small_t<112>(p, plan, s); break;
-    case 128: e = mc::launch_small_t<128>(p, plan, s); break;
-  }
-  if (e != cudaSuccess) return MC_CUDA;
-  if (plan.splits > 1)
-    e = mc::launch_attn_join(r, p.split, plan.tile_keys, 16 * plan.warps_rows, plan.row_tiles, s);
+  cudaError_t e = cudaErrorNotSupported;
+  if (mc::long_pays(a)) e = mc::launch_cross(p, mc::cross_plan(a, true), a->workspace, s);
+  if (e == cudaErrorNotSupported) e = mc::launch_cross(p, mc::cross_plan(a, false), a->workspace, s);
   return e == cudaSuccess ? MC_OK : MC_CUDA;
 }

@@ -1,0 +1,436 @@
+// cross_attn_long.cu -- mc_cross_attention for long sequences: tcgen05 MMAs
+// with accumulators in TMEM, fed by TMA.
+//
+// One CTA per unit (sequence, key/value head, 256 query rows) and key range.
+// Its rows are two tiles of 128, whose steps alternate on the tensor pipe:
+// while one tile's weights are computed, the other's products run.
+//   S_i [128 x 128 keys]  = Q_i K_j^T   (both K-major in shared memory)
+//   O_i [128 x head_dim] += W_i V_j     (W_i from TMEM, V_j as it lies, N-major)
+// Warp 0 loads K and V tiles through a ring, warp 1 issues the MMAs, warps
+// 4-7 and 8-11 hold one query row per thread of tile 0 and 1: they read S_i,
+// keep the row's maximum and sum, and write the weights, rounded to the
+// type, over S_i.  O_i is only rescaled when a maximum grows by more than 8
+// (in powers of two): the weights stay below 2^8 and exact in their ratio.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <cstring>
+
+#include "cross_attn.cuh"
+
+namespace mc {
+namespace {
+
+constexpr uint32_t kFull = 0xFFFFFFFFu;
+constexpr int kThreads = 384;
+constexpr int kTileBytes = 128 * 128;  // 128 rows of 64 channels
+constexpr float kGrowth = 8.0f;
+
+constexpr int chunks_of(int d) { return (d + 63) / 64; }
+constexpr int slots_of(int d) { return d > 64 ? 4 : 8; }
+constexpr int long_smem(int d) { return (2 + slots_of(d)) * chunks_of(d) * kTileBytes + 1024 + 256; }
+
+struct Barriers {
+  uint64_t full[8], empty[8];
+  uint64_t q_ready, s_full[2], w_ready[2], o_done[2], v_clean;
+  uint32_t tmem, stop;
+};
+
+// Bounded wait that also ends when another warp has given up.
+__device__ __forceinline__ bool wait_for(Barriers* b, uint64_t* bar, uint32_t phase, uint32_t* status) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if ((i & 63) == 63 && *reinterpret_cast<volatile uint32_t*>(&b->stop)) return false;
+  }
+  flag_status(status, kStatusWaitTimeout);
+  *reinterpret_cast<volatile uint32_t*>(&b->stop) = 1;
+  return false;
+}
+
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// B operand whose N (channels) is contiguous: 64-channel chunks `chunk` bytes
+// apart, groups of 8 keys 1,024 bytes apart, 128-byte swizzle.
+__device__ __forceinline__ uint64_t sdesc_n_sw128(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);
+  d |= (uint64_t)(kTileBytes >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// Instruction descriptor: 16-bit operands of one type, f32 sums, M = 128.
+__host__ __device__ constexpr uint32_t idesc_16(int n, bool bf16, bool b_n_major) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_n_major ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_long_kernel(const CrossParams p, const __grid_constant__ CUtensorMap k_map,
+                      const __grid_constant__ CUtensorMap v_map) {
+  constexpr int kChunks = chunks_of(D), kSlots = slots_of(D), kSteps = D / 16;
+  constexpr uint32_t kS0 = 0, kO0 = 256;  // TMEM columns: S_i at 128 i, O_i at 256 + 128 i
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_smem = smem;
+  uint8_t* ring = smem + 2 * kChunks * kTileBytes;
+  Barriers* bar = reinterpret_cast<Barriers*>(ring + kSlots * kChunks * kTileBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&bar->full[i], 1);
+      mbar_init(&bar->empty[i], 1);
+    }
+    mbar_init(&bar->q_ready, 256);
+    mbar_init(&bar->v_clean, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->w_ready[i], 128);
+      mbar_init(&bar->o_done[i], 1);
+    }
+    bar->stop = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bar->tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar->tmem;
+  pdl_enter();
+
+  const AttnRows& r = p.rows;
+  const long long unit = blockIdx.x, bh = unit / p.row_tiles;
+  const int tile = (int)(unit - bh * p.row_tiles), b = (int)(bh / r.kv_heads), head = (int)(bh - (long long)b * r.kv_heads);
+  const int split = blockIdx.y;
+  const AttnSeq seq = attn_seq(r, b, p.status, head == 0 && tile == 0 && split == 0 && threadIdx.x == 0);
+  const int n_rows = seq.nq * r.group, row0 = tile * kLongRows;
+  const int n_tiles = (seq.nk + kLongKeys - 1) / kLongKeys;
+  const int parts = max(1, (n_tiles + p.split.chunk - 1) / p.split.chunk);
+  const bool live = seq.ok && row0 < n_rows && split < parts;
+  const int begin = split * p.split.chunk, end = live ? min(n_tiles, begin + p.split.chunk) : begin;
+  const int steps = end - begin;
+  const int row_tiles = row0 + 128 < n_rows ? 2 : 1;
+  const int spare = steps > 0 ? max(0, end * kLongKeys - seq.nk) : 0;  // keys of the last tile behind the sequence
+
+  if (warp == 0 && steps > 0) {
+    // ---- loads: K_0, V_0, K_1, V_1, ... ----
+    bool ok = true;
+    int t = 0;
+    for (; ok && t < 2 * steps; ++t) {
+      const int slot = t % kSlots;
+      if (t >= kSlots) ok = __all_sync(kFull, wait_for(bar, &bar->empty[slot], (t / kSlots - 1) & 1, p.status));
+      if (!ok) break;
+      const int row = seq.k0 + (begin + t / 2) * kLongKeys;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bar->full[slot], kChunks * kTileBytes);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          tma_load_3d(ring + (slot * kChunks + c) * kTileBytes, t & 1 ? &v_map : &k_map, 64 * c,
+                      (t & 1 ? p.v_hs : p.k_hs) ? head : 0, row, &bar->full[slot]);
+      }
+      __syncwarp();
+    }
+    if (ok && spare) {
+      // The rows behind the sequence are the next one's, or anything: a
+      // weight of 0 times an infinity would be NaN.
+      const int last = 2 * steps - 1, slot = last % kSlots;
+      ok = __all_sync(kFull, wait_for(bar, &bar->full[slot], (last / kSlots) & 1, p.status));
+      uint8_t* v = ring + slot * kChunks * kTileBytes + (128 - spare) * 128;
+      for (int i = lane; i < spare * 8; i += 32)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) *reinterpret_cast<uint4*>(v + c * kTileBytes + i * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive(&bar->v_clean);
+    }
+    if (!ok)  // let the loads in flight land before the block leaves
+      for (int k = max(0, t - kSlots); k < t; ++k) {
+        for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&bar->full[k % kSlots], (k / kSlots) & 1); ++i) {
+        }
+      }
+  } else if (warp == 1 && lane == 0 && steps > 0) {
+    // ---- MMAs ----
+    constexpr uint32_t kIdescS = idesc_16(128, BF16, false), kIdescO = idesc_16(D, BF16, true);
+    auto scores = [&](int i, int j) {
+      const uint32_t q = smem_u32(q_smem + i * kChunks * kTileBytes);
+      const uint32_t k = smem_u32(ring + ((2 * j) % kSlots) * kChunks * kTileBytes);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t at = (s / 4) * kTileBytes + (s % 4) * 32;
+        mma_ss(tmem + kS0 + 128 * i, sdesc_k_sw128(q + at), sdesc_k_sw128(k + at), kIdescS, s > 0);
+      }
+      mma_commit(&bar->s_full[i]);
+    };
+    bool ok = wait_for(bar, &bar->q_ready, 0, p.status) && wait_for(bar, &bar->full[0], 0, p.status);
+    if (ok) {
+      tc_fence_after();
+      for (int i = 0; i < row_tiles; ++i) scores(i, 0);
+      mma_commit(&bar->empty[0]);
+    }
+    for (int j = 0; ok && j < steps; ++j) {
+      const int kt = 2 * (j + 1), vt = 2 * j + 1;
+      if (j + 1 < steps) ok = wait_for(bar, &bar->full[kt % kSlots], (kt / kSlots) & 1, p.status);
+      ok = ok && wait_for(bar, &bar->full[vt % kSlots], (vt / kSlots) & 1, p.status);
+      if (ok && j + 1 == steps && spare) ok = wait_for(bar, &bar->v_clean, 0, p.status);
+      for (int i = 0; ok && i < row_tiles; ++i) {
+        ok = wait_for(bar, &bar->w_ready[i], j & 1, p.status);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v = smem_u32(ring + (vt % kSlots) * kChunks * kTileBytes);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          mma_ts(tmem + kO0 + 128 * i, tmem + kS0 + 128 * i + 8 * s, sdesc_n_sw128(v + s * 2048), kIdescO, j > 0 || s > 0);
+        mma_commit(&bar->o_done[i]);
+        if (j + 1 < steps) scores(i, j + 1);
+      }
+      if (ok) {
+        mma_commit(&bar->empty[vt % kSlots]);
+        if (j + 1 < steps) mma_commit(&bar->empty[kt % kSlots]);
+      }
+    }
+    // the last arrival lands before the block, and its barriers, are gone
+    if (ok) wait_for(bar, &bar->empty[(2 * steps - 1) % kSlots], ((2 * steps - 1) / kSlots) & 1, p.status);
+  } else if (warp >= 4 && live) {
+    // ---- one query row per thread ----
+    const int i = (warp - 4) >> 2, quarter = warp & 3, row_in = quarter * 32 + lane, row = row0 + 128 * i + row_in;
+    const bool there = row < n_rows;
+    const int pos = there ? row / r.group : 0, h = head * r.group + (there ? row - pos * r.group : 0);
+    {
+      // the row of Q into its swizzled place: 16-byte chunk c of line l at c ^ (l % 8)
+      const uint16_t* src = static_cast<const uint16_t*>(r.q) + (long long)(seq.q0 + pos) * r.q_row_stride + (long long)h * r.q_head_stride;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 v = there ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(q_smem + (i * kChunks + c / 8) * kTileBytes + row_in * 128 + (((c & 7) ^ (row_in & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      arrive(&bar->q_ready);
+    }
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + kS0 + 128 * i, o_addr = tmem + lanes + kO0 + 128 * i;
+    const float factor = __fmul_rn(p.scale, kLog2e);
+    float top = -INFINITY, sum = 0.0f;
+    bool ok = steps > 0 && i < row_tiles;
+    for (int j = 0; ok && j < steps; ++j) {
+      ok = __all_sync(kFull, wait_for(bar, &bar->s_full[i], j & 1, p.status));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + 32 * c, s[c]);
+      tmem_ld_wait();
+      if (spare && j + 1 == steps) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (32 * c + k >= 128 - spare) s[c][k] = 0xFF800000u;
+      }
+      float most[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        most[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+        for (int k = 1; k < 32; ++k) most[c] = fmaxf(most[c], __uint_as_float(s[c][k]));
+      }
+      const float high = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+      if (__any_sync(kFull, __fmul_rn(__fsub_rn(high, top), factor) > kGrowth)) {
+        const float grown = fmaxf(top, high);
+        const float shrink = top == -INFINITY ? 0.0f : exp2_approx(__fmul_rn(__fsub_rn(top, grown), factor));
+        top = grown;
+        sum = __fmul_rn(sum, shrink);
+        if (j > 0) {
+          ok = __all_sync(kFull, wait_for(bar, &bar->o_done[i], (j - 1) & 1, p.status));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_x16(o_addr + 16 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__fmul_rn(__uint_as_float(o[k]), shrink));
+            tmem_st_x16(o_addr + 16 * c, o);
+          }
+        }
+      }
+      const float base = top == -INFINITY ? 0.0f : __fmul_rn(-top, factor);
+      float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float a = exp2_approx(__fmaf_rn(__uint_as_float(s[c][2 * k]), factor, base));
+          const float e = exp2_approx(__fmaf_rn(__uint_as_float(s[c][2 * k + 1]), factor, base));
+          add[k & 3] = __fadd_rn(add[k & 3], __fadd_rn(a, e));
+          w[k] = BF16 ? pack_bf16(a, e) : pack_f16(a, e);
+        }
+        tmem_st_x16(s_addr + 16 * c, w);
+      }
+      sum = __fadd_rn(sum, __fadd_rn(__fadd_rn(add[0], add[1]), __fadd_rn(add[2], add[3])));
+      tmem_st_wait();
+      tc_fence_before();
+      arrive(&bar->w_ready[i]);
+    }
+    if (ok) ok = __all_sync(kFull, wait_for(bar, &bar->o_done[i], (steps - 1) & 1, p.status));
+    const bool written = i < row_tiles && (ok || steps <= 0);
+    // ---- the row, normalized ----
+    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    const float lse2 = sum == 0.0f ? -INFINITY : __fadd_rn(__fmul_rn(top, factor), log2f(sum));
+    const bool direct = parts <= 1;
+    const long long slot = (unit * kLongRows + 128 * i + row_in) * p.split.splits + split;
+    if (ok) tc_fence_after();
+    if (__any_sync(kFull, written && there)) {
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16];
+        __syncwarp();
+        if (ok) {
+          tmem_ld_x16(o_addr + 16 * c, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = 0;
+        }
+        float f[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) f[k] = __fmul_rn(__uint_as_float(o[k]), inv);
+        if (direct && written && there) {
+          uint32_t w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = BF16 ? pack_bf16(f[2 * k], f[2 * k + 1]) : pack_f16(f[2 * k], f[2 * k + 1]);
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(r.out) + (long long)(seq.q0 + pos) * r.out_row_stride +
+                                                (long long)h * r.out_head_stride + 16 * c);
+          dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else if (written && there) {
+          float4* dst = reinterpret_cast<float4*>(p.split.out + slot * D + 16 * c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dst[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+        }
+      }
+      if (written && there) {
+        if (!direct)
+          p.split.lse[slot] = lse2;
+        else if (r.lse)
+          r.lse[(long long)(seq.q0 + pos) * r.kv_heads * r.group + h] = __fmul_rn(lse2, kLn2);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    void* ptr = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }
+  return fn;
+}
+
+// {channels, heads, rows} of k or v, boxes of 64 channels of one head and 128
+// rows; channels past head_dim and rows past the last come as zeros.  Heads
+// that share one row (a stride of 0) are one head there.
+bool encode_rows(CUtensorMap* map, const void* base, const AttnRows& r, long long row_stride, long long head_stride) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)r.head_dim, (cuuint64_t)(head_stride ? r.kv_heads : 1), (cuuint64_t)r.k_rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)(head_stride ? head_stride : r.head_dim) * 2, (cuuint64_t)row_stride * 2};
+  const cuuint32_t box[3] = {64, 1, kLongKeys}, steps[3] = {1, 1, 1};
+  return fn(map, r.dtype == MC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16>
+cudaError_t launch_long(const CrossParams& p, long long units, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
+  static uint64_t done = 0;
+  cudaError_t e = allow_smem(cross_long_kernel<D, BF16>, long_smem(D), &done);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(cross_long_kernel<D, BF16>, dim3((unsigned)units, p.split.splits), dim3(kThreads), long_smem(D), s, p, k, v);
+}
+
+template <int D>
+cudaError_t launch_long_t(const CrossParams& p, long long units, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
+  return p.rows.dtype == MC_BF16 ? launch_long<D, true>(p, units, k, v, s) : launch_long<D, false>(p, units, k, v, s);
+}
+
+}  // namespace
+
+bool cross_long_strides(const mc_cross_attention_args* a) {
+  return a->k_rows > 0 && a->k_row_stride >= a->head_dim && a->v_row_stride >= a->head_dim;
+}
+
+cudaError_t launch_cross_long(const CrossParams& p, long long units, cudaStream_t s) {
+  CUtensorMap k, v;
+  if (!encode_rows(&k, p.k, p.rows, p.k_rs, p.k_hs) || !encode_rows(&v, p.v, p.rows, p.v_rs, p.v_hs))
+    return cudaErrorNotSupported;
+  switch (p.rows.head_dim) {
+    case 16: return launch_long_t<16>(p, units, k, v, s);
+    case 32: return launch_long_t<32>(p, units, k, v, s);
+    case 48: return launch_long_t<48>(p, units, k, v, s);
+    case 64: return launch_long_t<64>(p, units, k, v, s);
+    case 80: return launch_long_t<80>(p, units, k, v, s);
+    case 96: return launch_long_t<96>(p, units, k, v, s);
+    case 112: return launch_long_t<112>(p, units, k, v, s);
+    case 128: return launch_long_t<128>(p, units, k, v, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace mc
