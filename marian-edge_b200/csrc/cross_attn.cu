@@ -453,11 +453,12 @@ bool cross_sizes_ok(const mc_cross_attention_args* a) {
          (int64_t)a->batch * a->kv_heads * ((int64_t)(a->heads / a->kv_heads) * a->max_q_len / 16 + 1) <= INT32_MAX;
 }
 
-// Long tiles pay where a sequence's rows fill most of two of them and its keys
-// a few: below, the small kernel's 16-row warps waste less.
+// Long tiles pay where the sequences' rows fill one of two on average: below,
+// the small kernel's 16-row warps waste less.
 bool long_pays(const mc_cross_attention_args* a) {
+  const int64_t mean = a->batch > 0 ? a->q_rows / a->batch : 0, group = a->heads / a->kv_heads;
   return a->dtype != MC_F32 && !a->key_mask && a->scale > 0.0f && cross_long_strides(a) &&
-         (int64_t)(a->heads / a->kv_heads) * a->max_q_len >= 128 && a->max_k_len >= 128;
+         group * (mean < a->max_q_len ? mean : a->max_q_len) >= 128 && a->max_k_len >= 128;
 }
 
 CrossPlan cross_plan(const mc_cross_attention_args* a, bool long_tiles) {

@@ -25,14 +25,20 @@ constexpr uint32_t kFull = 0xFFFFFFFFu;
 constexpr int kThreads = 384;
 constexpr int kTileBytes = 128 * 128;  // 128 rows of 64 channels
 constexpr float kGrowth = 8.0f;
+// Of the weights' exponentials, one pair in kPolyEvery is computed on the FMA
+// pipe: the special-function unit (16 a cycle) would take as long for a tile's
+// 16,384 as the tensor cores for both its products.
+constexpr int kPolyEvery = 4;
 
 constexpr int chunks_of(int d) { return (d + 63) / 64; }
-constexpr int slots_of(int d) { return d > 64 ? 4 : 8; }
-constexpr int long_smem(int d) { return (2 + slots_of(d)) * chunks_of(d) * kTileBytes + 1024 + 256; }
+// Ring stages, each for the V tile of one step and the K tile of the next,
+// which the MMAs of a step read together.
+constexpr int stages_of(int d) { return d > 64 ? 2 : 4; }
+constexpr int long_smem(int d) { return (2 + 2 * stages_of(d)) * chunks_of(d) * kTileBytes + 1024 + 256; }
 
 struct Barriers {
-  uint64_t full[8], empty[8];
-  uint64_t q_ready, s_full[2], w_ready[2], o_done[2], v_clean;
+  uint64_t full[4], empty[4];
+  uint64_t k0_full, k0_done, q_ready, s_full[2], w_ready[2][2], o_done[2], v_clean;
   uint32_t tmem, stop;
 };
 
@@ -45,6 +51,14 @@ __device__ __forceinline__ bool wait_for(Barriers* b, uint64_t* bar, uint32_t ph
   flag_status(status, kStatusWaitTimeout);
   *reinterpret_cast<volatile uint32_t*>(&b->stop) = 1;
   return false;
+}
+
+// The same for a whole warp, of which one lane polls: thirty-two lanes on one
+// barrier keep its unit from the arrivals of others.
+__device__ __forceinline__ bool warp_wait(Barriers* b, uint64_t* bar, uint32_t phase, uint32_t* status) {
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0) ok = wait_for(b, bar, phase, status);
+  return __all_sync(kFull, ok);
 }
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {
@@ -67,6 +81,15 @@ __device__ __forceinline__ uint64_t sdesc_n_sw128(uint32_t addr) {
 __host__ __device__ constexpr uint32_t idesc_16(int n, bool bf16, bool b_n_major) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_n_major ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// True in one lane of a converged warp.  MMAs are issued under it by warps
+// that run their control flow whole: their descriptors then stay in uniform
+// registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -102,31 +125,81 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t addr, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---- pairs of f32 (one instruction, two lanes) ----
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t d, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of a pair on the FMA pipe: x = n + f, n whole (adding 1.5 * 2^23 rounds),
+// 2^f by the polynomial of degree 5 with the least largest relative error on
+// [-1/2, 1/2] (8e-8), n added to its exponent.  x below -126 counts as -126.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
+  float a, b;
+  unpair(x2, a, b);
+  x2 = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const uint64_t magic = pair(12582912.0f, 12582912.0f), t = add2(x2, magic);
+  const uint64_t n = add2(t, pair(-12582912.0f, -12582912.0f));
+  const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x2);
+  uint64_t y = fma2(f, pair(0.0013276472f, 0.0013276472f), pair(0.009675541f, 0.009675541f));
+  y = fma2(f, y, pair(0.05550713f, 0.05550713f));
+  y = fma2(f, y, pair(0.2402212f, 0.2402212f));
+  y = fma2(f, y, pair(0.69314694f, 0.69314694f));
+  y = fma2(f, y, pair(1.0000001f, 1.0000001f));
+  float u, v;
+  unpair(t, u, v);
+  unpair(y, a, b);
+  return pair(__uint_as_float(__float_as_uint(a) + (__float_as_uint(u) << 23)),
+              __uint_as_float(__float_as_uint(b) + (__float_as_uint(v) << 23)));
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_long_kernel(const CrossParams p, const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map) {
-  constexpr int kChunks = chunks_of(D), kSlots = slots_of(D), kSteps = D / 16;
+  constexpr int kChunks = chunks_of(D), kStages = stages_of(D), kSteps = D / 16;
   constexpr uint32_t kS0 = 0, kO0 = 256;  // TMEM columns: S_i at 128 i, O_i at 256 + 128 i
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = smem;
   uint8_t* ring = smem + 2 * kChunks * kTileBytes;
-  Barriers* bar = reinterpret_cast<Barriers*>(ring + kSlots * kChunks * kTileBytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Barriers* bar = reinterpret_cast<Barriers*>(ring + 2 * kStages * kChunks * kTileBytes);
+  const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&k_map);
     tma_prefetch_desc(&v_map);
-    for (int i = 0; i < kSlots; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&bar->full[i], 1);
       mbar_init(&bar->empty[i], 1);
     }
-    mbar_init(&bar->q_ready, 256);
+    mbar_init(&bar->k0_full, 1);
+    mbar_init(&bar->k0_done, 1);
+    mbar_init(&bar->q_ready, 8);
     mbar_init(&bar->v_clean, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->s_full[i], 1);
-      mbar_init(&bar->w_ready[i], 128);
+      mbar_init(&bar->w_ready[i][0], 4);
+      mbar_init(&bar->w_ready[i][1], 4);
       mbar_init(&bar->o_done[i], 1);
     }
     bar->stop = 0;
@@ -139,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar->tmem;
+  const uint32_t tmem = __shfl_sync(kFull, bar->tmem, 0);
   pdl_enter();
 
   const AttnRows& r = p.rows;
@@ -157,29 +230,38 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int spare = steps > 0 ? max(0, end * kLongKeys - seq.nk) : 0;  // keys of the last tile behind the sequence
 
   if (warp == 0 && steps > 0) {
-    // ---- loads: K_0, V_0, K_1, V_1, ... ----
-    bool ok = true;
-    int t = 0;
-    for (; ok && t < 2 * steps; ++t) {
-      const int slot = t % kSlots;
-      if (t >= kSlots) ok = __all_sync(kFull, wait_for(bar, &bar->empty[slot], (t / kSlots - 1) & 1, p.status));
-      if (!ok) break;
-      const int row = seq.k0 + (begin + t / 2) * kLongKeys;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bar->full[slot], kChunks * kTileBytes);
+    // ---- loads: K_0 (where the last stage's K goes later), then V_j with K_{j+1} ----
+    constexpr int kPart = kChunks * kTileBytes;  // a stage: V, then K
+    auto load = [&](uint8_t* to, const CUtensorMap* map, bool by_head, int step, uint64_t* full) {
+      const int row = seq.k0 + (begin + step) * kLongKeys;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-          tma_load_3d(ring + (slot * kChunks + c) * kTileBytes, t & 1 ? &v_map : &k_map, 64 * c,
-                      (t & 1 ? p.v_hs : p.k_hs) ? head : 0, row, &bar->full[slot]);
+      for (int c = 0; c < kChunks; ++c) tma_load_3d(to + c * kTileBytes, map, 64 * c, by_head ? head : 0, row, full);
+    };
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&bar->k0_full, kPart);
+      load(ring + (2 * kStages - 1) * kPart, &k_map, p.k_hs != 0, 0, &bar->k0_full);
+    }
+    bool ok = true;
+    int j = 0;
+    for (; j < steps; ++j) {
+      const int st = j % kStages;
+      if (j >= kStages) ok = warp_wait(bar, &bar->empty[st], (j / kStages - 1) & 1, p.status);
+      if (ok && j == kStages - 1) ok = warp_wait(bar, &bar->k0_done, 0, p.status);
+      if (!ok) break;
+      if (lane == 0) {
+        const bool more = j + 1 < steps;
+        mbar_arrive_expect_tx(&bar->full[st], more ? 2 * kPart : kPart);
+        load(ring + 2 * st * kPart, &v_map, p.v_hs != 0, j, &bar->full[st]);
+        if (more) load(ring + (2 * st + 1) * kPart, &k_map, p.k_hs != 0, j + 1, &bar->full[st]);
       }
       __syncwarp();
     }
     if (ok && spare) {
       // The rows behind the sequence are the next one's, or anything: a
       // weight of 0 times an infinity would be NaN.
-      const int last = 2 * steps - 1, slot = last % kSlots;
-      ok = __all_sync(kFull, wait_for(bar, &bar->full[slot], (last / kSlots) & 1, p.status));
-      uint8_t* v = ring + slot * kChunks * kTileBytes + (128 - spare) * 128;
+      const int st = (steps - 1) % kStages;
+      ok = warp_wait(bar, &bar->full[st], ((steps - 1) / kStages) & 1, p.status);
+      uint8_t* v = ring + 2 * st * kPart + (128 - spare) * 128;
       for (int i = lane; i < spare * 8; i += 32)
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) *reinterpret_cast<uint4*>(v + c * kTileBytes + i * 16) = make_uint4(0, 0, 0, 0);
@@ -187,53 +269,85 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) arrive(&bar->v_clean);
     }
-    if (!ok)  // let the loads in flight land before the block leaves
-      for (int k = max(0, t - kSlots); k < t; ++k) {
-        for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&bar->full[k % kSlots], (k / kSlots) & 1); ++i) {
+    if (!ok) {  // let the loads in flight land before the block leaves
+      for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&bar->k0_full, 0); ++i) {
+      }
+      for (int k = max(0, j - kStages); k < min(j, steps); ++k)
+        for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&bar->full[k % kStages], (k / kStages) & 1); ++i) {
         }
-      }
-  } else if (warp == 1 && lane == 0 && steps > 0) {
+    }
+  } else if (warp == 1 && steps > 0) {
     // ---- MMAs ----
+    // One lane issues them all, and the tensor pipe waits for it: every
+    // descriptor is a base plus a constant (16-byte units; shared memory
+    // addresses need no carry), and the next stage is waited for while the
+    // pipe has tile 0's products before it.  An arrival on s_full also says
+    // that the tile's product before it is done, as one thread's MMAs are.
     constexpr uint32_t kIdescS = idesc_16(128, BF16, false), kIdescO = idesc_16(D, BF16, true);
-    auto scores = [&](int i, int j) {
-      const uint32_t q = smem_u32(q_smem + i * kChunks * kTileBytes);
-      const uint32_t k = smem_u32(ring + ((2 * j) % kSlots) * kChunks * kTileBytes);
+    constexpr uint32_t kPart = kChunks * kTileBytes / 16;
+    const int n = __shfl_sync(kFull, steps, 0), tiles = __shfl_sync(kFull, row_tiles, 0);
+    const bool cut = __shfl_sync(kFull, spare, 0) > 0;
+    const uint64_t q_desc = sdesc_k_sw128(smem_u32(q_smem)), k_desc = sdesc_k_sw128(smem_u32(ring)),
+                   v_desc = sdesc_n_sw128(smem_u32(ring));
+    auto scores = [&](int i, int stage) {
+      const uint64_t q = q_desc + i * kPart, k = k_desc + (2 * stage + 1) * kPart;
+      const uint32_t d = tmem + kS0 + 128 * i;
+      if (elect_one()) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const uint32_t at = (s / 4) * kTileBytes + (s % 4) * 32;
-        mma_ss(tmem + kS0 + 128 * i, sdesc_k_sw128(q + at), sdesc_k_sw128(k + at), kIdescS, s > 0);
+        for (int s = 0; s < kSteps; ++s) {
+          const uint32_t at = ((s / 4) * kTileBytes + (s % 4) * 32) / 16;
+          mma_ss(d, q + at, k + at, kIdescS, s > 0);
+        }
+        mma_commit(&bar->s_full[i]);
       }
-      mma_commit(&bar->s_full[i]);
+      __syncwarp();
     };
-    bool ok = wait_for(bar, &bar->q_ready, 0, p.status) && wait_for(bar, &bar->full[0], 0, p.status);
+    auto commit = [&](uint64_t* b) {
+      if (elect_one()) mma_commit(b);
+      __syncwarp();
+    };
+    auto stage_ready = [&](int j) {
+      bool ok = warp_wait(bar, &bar->full[j % kStages], (j / kStages) & 1, p.status);
+      if (ok && j + 1 == n && cut) ok = warp_wait(bar, &bar->v_clean, 0, p.status);
+      return ok;
+    };
+    bool ok = warp_wait(bar, &bar->q_ready, 0, p.status) && warp_wait(bar, &bar->k0_full, 0, p.status);
     if (ok) {
       tc_fence_after();
-      for (int i = 0; i < row_tiles; ++i) scores(i, 0);
-      mma_commit(&bar->empty[0]);
+      for (int i = 0; i < tiles; ++i) scores(i, kStages - 1);
+      commit(&bar->k0_done);
+      ok = stage_ready(0);
     }
-    for (int j = 0; ok && j < steps; ++j) {
-      const int kt = 2 * (j + 1), vt = 2 * j + 1;
-      if (j + 1 < steps) ok = wait_for(bar, &bar->full[kt % kSlots], (kt / kSlots) & 1, p.status);
-      ok = ok && wait_for(bar, &bar->full[vt % kSlots], (vt / kSlots) & 1, p.status);
-      if (ok && j + 1 == steps && spare) ok = wait_for(bar, &bar->v_clean, 0, p.status);
-      for (int i = 0; ok && i < row_tiles; ++i) {
-        ok = wait_for(bar, &bar->w_ready[i], j & 1, p.status);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t v = smem_u32(ring + (vt % kSlots) * kChunks * kTileBytes);
+    for (int j = 0; ok && j < n; ++j) {
+      const int st = j % kStages;
+      const uint64_t v = v_desc + 2 * st * kPart;
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          mma_ts(tmem + kO0 + 128 * i, tmem + kS0 + 128 * i + 8 * s, sdesc_n_sw128(v + s * 2048), kIdescO, j > 0 || s > 0);
-        mma_commit(&bar->o_done[i]);
-        if (j + 1 < steps) scores(i, j + 1);
+      for (int i = 0; i < 2; ++i) {
+        if (i >= tiles || !ok) break;
+        const uint32_t d = tmem + kO0 + 128 * i, w = tmem + kS0 + 128 * i;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // the first 64 keys while the others' weights are made
+          if (ok) ok = warp_wait(bar, &bar->w_ready[i][half], j & 1, p.status);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              mma_ts(d, w + 8 * (4 * half + s), v + (4 * half + s) * 128, kIdescO, j > 0 || half > 0 || s > 0);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (j + 1 < n)
+          scores(i, st);
+        else
+          commit(&bar->o_done[i]);
+        if (i == 0 && j + 1 < n) ok = stage_ready(j + 1);
       }
-      if (ok) {
-        mma_commit(&bar->empty[vt % kSlots]);
-        if (j + 1 < steps) mma_commit(&bar->empty[kt % kSlots]);
-      }
+      if (ok) commit(&bar->empty[st]);
     }
     // the last arrival lands before the block, and its barriers, are gone
-    if (ok) wait_for(bar, &bar->empty[(2 * steps - 1) % kSlots], ((2 * steps - 1) / kSlots) & 1, p.status);
+    if (ok) warp_wait(bar, &bar->empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, p.status);
   } else if (warp >= 4 && live) {
     // ---- one query row per thread ----
     const int i = (warp - 4) >> 2, quarter = warp & 3, row_in = quarter * 32 + lane, row = row0 + 128 * i + row_in;
@@ -248,7 +362,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reinterpret_cast<uint4*>(q_smem + (i * kChunks + c / 8) * kTileBytes + row_in * 128 + (((c & 7) ^ (row_in & 7)) << 4)) = v;
       }
       fence_proxy_async_smem();
-      arrive(&bar->q_ready);
+      __syncwarp();
+      if (lane == 0) arrive(&bar->q_ready);
     }
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lanes + kS0 + 128 * i, o_addr = tmem + lanes + kO0 + 128 * i;
@@ -256,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float top = -INFINITY, sum = 0.0f;
     bool ok = steps > 0 && i < row_tiles;
     for (int j = 0; ok && j < steps; ++j) {
-      ok = __all_sync(kFull, wait_for(bar, &bar->s_full[i], j & 1, p.status));
+      ok = warp_wait(bar, &bar->s_full[i], j & 1, p.status);
       if (!ok) break;
       tc_fence_after();
       uint32_t s[4][32];
@@ -273,20 +388,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       float most[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        most[c] = __uint_as_float(s[c][0]);
+        most[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
 #pragma unroll
-        for (int k = 1; k < 32; ++k) most[c] = fmaxf(most[c], __uint_as_float(s[c][k]));
+        for (int k = 2; k < 32; k += 2) most[c] = max3(most[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       }
-      const float high = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+      const float high = max3(fmaxf(most[0], most[1]), most[2], most[3]);
       if (__any_sync(kFull, __fmul_rn(__fsub_rn(high, top), factor) > kGrowth)) {
         const float grown = fmaxf(top, high);
         const float shrink = top == -INFINITY ? 0.0f : exp2_approx(__fmul_rn(__fsub_rn(top, grown), factor));
         top = grown;
         sum = __fmul_rn(sum, shrink);
         if (j > 0) {
-          ok = __all_sync(kFull, wait_for(bar, &bar->o_done[i], (j - 1) & 1, p.status));
-          if (!ok) break;
-          tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
@@ -299,25 +411,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float base = top == -INFINITY ? 0.0f : __fmul_rn(-top, factor);
-      float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint64_t factor2 = pair(factor, factor), base2 = pair(base, base);
+      uint64_t add[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float a = exp2_approx(__fmaf_rn(__uint_as_float(s[c][2 * k]), factor, base));
-          const float e = exp2_approx(__fmaf_rn(__uint_as_float(s[c][2 * k + 1]), factor, base));
-          add[k & 3] = __fadd_rn(add[k & 3], __fadd_rn(a, e));
+          uint64_t x = fma2(pair(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1])), factor2, base2);
+          float a, e;
+          if (k % kPolyEvery == kPolyEvery - 1) {
+            x = exp2_pair(x);
+            unpair(x, a, e);
+          } else {
+            unpair(x, a, e);
+            a = exp2_approx(a);
+            e = exp2_approx(e);
+            x = pair(a, e);
+          }
+          add[k & 1] = add2(add[k & 1], x);
           w[k] = BF16 ? pack_bf16(a, e) : pack_f16(a, e);
         }
         tmem_st_x16(s_addr + 16 * c, w);
+        if (c & 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive(&bar->w_ready[i][c >> 1]);
+        }
       }
-      sum = __fadd_rn(sum, __fadd_rn(__fadd_rn(add[0], add[1]), __fadd_rn(add[2], add[3])));
-      tmem_st_wait();
-      tc_fence_before();
-      arrive(&bar->w_ready[i]);
+      float a0, a1;
+      unpair(add2(add[0], add[1]), a0, a1);
+      sum = __fadd_rn(sum, __fadd_rn(a0, a1));
     }
-    if (ok) ok = __all_sync(kFull, wait_for(bar, &bar->o_done[i], (steps - 1) & 1, p.status));
+    if (ok) ok = warp_wait(bar, &bar->o_done[i], 0, p.status);
     const bool written = i < row_tiles && (ok || steps <= 0);
     // ---- the row, normalized ----
     const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
