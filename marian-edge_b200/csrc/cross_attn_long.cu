@@ -53,8 +53,9 @@ __device__ __forceinline__ bool wait_for(Barriers* b, uint64_t* bar, uint32_t ph
   return false;
 }
 
-// The same for a whole warp, of which one lane polls: thirty-two lanes on one
-// barrier keep its unit from the arrivals of others.
+// The same for a whole warp, of which one lane polls, for waits that are
+// mostly long.  (The MMA warp's are short, and a lane's return costs more
+// there than the others' polling: 609 us against 580 at 2 x 4,096 x 8,192.)
 __device__ __forceinline__ bool warp_wait(Barriers* b, uint64_t* bar, uint32_t phase, uint32_t* status) {
   bool ok = true;
   if ((threadIdx.x & 31) == 0) ok = wait_for(b, bar, phase, status);
@@ -307,11 +308,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     };
     auto stage_ready = [&](int j) {
-      bool ok = warp_wait(bar, &bar->full[j % kStages], (j / kStages) & 1, p.status);
-      if (ok && j + 1 == n && cut) ok = warp_wait(bar, &bar->v_clean, 0, p.status);
-      return ok;
+      bool ok = wait_for(bar, &bar->full[j % kStages], (j / kStages) & 1, p.status);
+      if (ok && j + 1 == n && cut) ok = wait_for(bar, &bar->v_clean, 0, p.status);
+      return (bool)__all_sync(kFull, ok);
     };
-    bool ok = warp_wait(bar, &bar->q_ready, 0, p.status) && warp_wait(bar, &bar->k0_full, 0, p.status);
+    bool ok = __all_sync(kFull, wait_for(bar, &bar->q_ready, 0, p.status) && wait_for(bar, &bar->k0_full, 0, p.status));
     if (ok) {
       tc_fence_after();
       for (int i = 0; i < tiles; ++i) scores(i, kStages - 1);
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t d = tmem + kO0 + 128 * i, w = tmem + kS0 + 128 * i;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {  // the first 64 keys while the others' weights are made
-          if (ok) ok = warp_wait(bar, &bar->w_ready[i][half], j & 1, p.status);
+          ok = __all_sync(kFull, ok && wait_for(bar, &bar->w_ready[i][half], j & 1, p.status));
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) commit(&bar->empty[st]);
     }
     // the last arrival lands before the block, and its barriers, are gone
-    if (ok) warp_wait(bar, &bar->empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, p.status);
+    if (ok) wait_for(bar, &bar->empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, p.status);
   } else if (warp >= 4 && live) {
     // ---- one query row per thread ----
     const int i = (warp - 4) >> 2, quarter = warp & 3, row_in = quarter * 32 + lane, row = row0 + 128 * i + row_in;

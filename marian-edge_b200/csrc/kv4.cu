@@ -12,6 +12,7 @@
 // as the difference of two sums tens of times their size (measured: f32
 // outputs 9e-6 off instead of 2e-7).
 #include <cstring>
+#include <type_traits>
 
 #include "decode_ops.cuh"
 
@@ -32,87 +33,152 @@ struct Kv4Pool {
 __host__ __device__ __forceinline__ int head_block(int tokens, int head_dim) { return tokens * (head_dim + 8); }
 
 // ---- append and read ---------------------------------------------------------------
-// One group of L lanes per row (L the power of two that holds head_dim / 8
-// lanes of 8 values), kRowsPerPass rows in flight per group so that their
-// loads overlap.  The rows of a CTA's 16 tokens are taken token by token for
-// one head, then the next: neighbouring groups write neighbouring code rows
-// and (scale, minimum) pairs of a page.
+// A CTA takes up to 32 tokens of a sequence.  A group of L lanes (the power of
+// two that holds head_dim / 8 lanes of 8 values) takes a head's key or value
+// rows, token after token, four rows in flight.
 struct Kv4RowsDev {
   void *k, *v;
   const int32_t *start, *count, *first;
   long long rows;
   long long k_rs, k_hs, v_rs, v_hs;
-  int dtype, max_count;
+  int max_count;
 };
 
 constexpr int kRowThreads = 256;
-constexpr int kRowTokens = 16;
-constexpr int kRowsPerPass = 4;
+constexpr int kRowTokens = 32;
+constexpr int kRowsInFlight = 4;
 
-struct RowAt {
-  uint8_t* codes;
-  __half2* params;
-  char* x;
-};
-
-__device__ __forceinline__ bool load_eight(const char* x, int dtype, float (&f)[8]) {
-  if (dtype == MC_F32) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(x));
-    const float4 b = __ldcs(reinterpret_cast<const float4*>(x) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(x));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// Eight neighbouring values of a row, as they lie in memory.
+template <int TYPE>
+struct Eight {
+  uint32_t w[TYPE == MC_F32 ? 8 : 4];
+  __device__ __forceinline__ void load(const char* x) {
+#pragma unroll
+    for (int i = 0; i < (TYPE == MC_F32 ? 2 : 1); ++i) {
+      const uint4 a = __ldcs(reinterpret_cast<const uint4*>(x) + i);
+      w[4 * i] = a.x;
+      w[4 * i + 1] = a.y;
+      w[4 * i + 2] = a.z;
+      w[4 * i + 3] = a.w;
+    }
+  }
+  __device__ __forceinline__ void values(float (&f)[8]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 t = dtype == MC_F16 ? unpack_f16(w[i]) : unpack_bf16(w[i]);
+      const float2 t = TYPE == MC_F32   ? make_float2(__uint_as_float(w[(2 * i) % (TYPE == MC_F32 ? 8 : 4)]),
+                                                      __uint_as_float(w[(2 * i + 1) % (TYPE == MC_F32 ? 8 : 4)]))
+                       : TYPE == MC_F16 ? unpack_f16(w[i])
+                                        : unpack_bf16(w[i]);
       f[2 * i] = t.x;
       f[2 * i + 1] = t.y;
     }
   }
-  return true;
-}
+};
 
-__device__ __forceinline__ void store_eight(char* x, int dtype, const float (&f)[8]) {
-  if (dtype == MC_F32) {
+template <int TYPE>
+__device__ __forceinline__ void store_eight(char* x, const float (&f)[8]) {
+  if (TYPE == MC_F32) {
     __stcs(reinterpret_cast<float4*>(x), make_float4(f[0], f[1], f[2], f[3]));
     __stcs(reinterpret_cast<float4*>(x) + 1, make_float4(f[4], f[5], f[6], f[7]));
   } else {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      w[i] = dtype == MC_F16 ? pack_f16(f[2 * i], f[2 * i + 1]) : pack_bf16(f[2 * i], f[2 * i + 1]);
+      w[i] = TYPE == MC_F16 ? pack_f16(f[2 * i], f[2 * i + 1]) : pack_bf16(f[2 * i], f[2 * i + 1]);
     __stcs(reinterpret_cast<uint4*>(x), make_uint4(w[0], w[1], w[2], w[3]));
   }
 }
 
-template <int L>
-__device__ __forceinline__ float group_min(float v) {
+// The smallest and largest of the row's values over L lanes; smallest -inf
+// when one of them is not finite (0 x it is NaN then).
+template <int TYPE, int L>
+__device__ __forceinline__ void row_range(const Eight<TYPE>& x, bool live, float* low, float* high) {
+  if (TYPE == MC_F32) {
+    float lo = INFINITY, hi = -INFINITY, z = 0.0f;
+    if (live) {
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(kFull, v, o));
-  return v;
-}
-template <int L>
-__device__ __forceinline__ float group_max(float v) {
+      for (int i = 0; i < 8; ++i) {
+        const float f = __uint_as_float(x.w[i % (TYPE == MC_F32 ? 8 : 4)]);
+        lo = fminf(lo, f);
+        hi = fmaxf(hi, f);
+        z = __fmaf_rn(f, 0.0f, z);
+      }
+      if (z != z) lo = -INFINITY;
+    }
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
-  return v;
+    for (int o = L / 2; o > 0; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
+    }
+    *low = lo;
+    *high = hi;
+  } else {
+    // both at once: the 16-bit pair (smallest, -largest), whose minimum is taken
+    using T2 = typename std::conditional<TYPE == MC_F16, __half2, __nv_bfloat162>::type;
+    auto as2 = [](uint32_t w) { return *reinterpret_cast<T2*>(&w); };
+    auto bits = [](T2 v) { return *reinterpret_cast<uint32_t*>(&v); };
+    const uint32_t inf = TYPE == MC_F16 ? 0x7C007C00u : 0x7F807F80u;
+    uint32_t both = inf;
+    if (live) {
+      T2 lo = as2(x.w[0]), hi = lo, z = __hmul2(lo, as2(0u));
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        lo = __hmin2(lo, as2(x.w[i]));
+        hi = __hmax2(hi, as2(x.w[i]));
+        z = __hfma2(as2(x.w[i]), as2(0u), z);
+      }
+      const uint32_t l = bits(lo), h = bits(hi) ^ 0x80008000u;
+      // (low halves, high halves) of both, then their minimum
+      both = bits(__hmin2(as2(__byte_perm(l, h, 0x5410)), as2(__byte_perm(l, h, 0x7632))));
+      const uint32_t zb = bits(z) & 0x7FFF7FFFu;
+      if (zb) both = inf | 0x80008000u;  // a NaN there, as 0 x finite has no bits left: (-inf, -inf)
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) both = bits(__hmin2(as2(both), as2(__shfl_xor_sync(kFull, both, o))));
+    const float2 t = TYPE == MC_F16 ? unpack_f16(both) : unpack_bf16(both);
+    *low = t.x;
+    *high = -t.y;
+  }
 }
 
-// The code of x: round((x - minimum) / scale) of the real quotient.  A
-// single-precision quotient is within 4e-6 of it for codes up to 16, so only
-// one that lands that near to a half needs the double-precision one, whose
-// ties are exact (the scale has 11 significant bits).
-__device__ __forceinline__ uint32_t code_of(float x, float minimum, float scale, float inverse) {
-  float t = __fmul_rn(__fsub_rn(x, minimum), inverse);
-  float c = rintf(t);
-  if (fabsf(__fsub_rn(t, c)) > 0.4999f)
-    c = (float)rint(__ddiv_rn(__dsub_rn((double)x, (double)minimum), (double)scale));
-  return (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f);
+// The codes of eight values: round((x - minimum) / scale) of the real
+// quotient.  A single-precision quotient is within 3e-6 of it for codes up to
+// 16, so only one that lands within 1e-5 of a half needs the double-precision
+// one, whose ties are exact (the scale has 11 significant bits).  Rounding is
+// the addition of 1.5 * 2^23; four codes are one exact float.
+__device__ __forceinline__ uint32_t codes_of(const float (&f)[8], float minimum, float scale) {
+  const float inverse = __frcp_rn(scale);
+  float c[8];
+  bool near_half = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(f[i], minimum), inverse), 0.0f), 15.0f);
+    c[i] = __fsub_rn(__fadd_rn(t, 12582912.0f), 12582912.0f);
+    near_half |= fabsf(__fsub_rn(t, c[i])) > 0.49999f;
+  }
+  if (near_half) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      float x = f[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) x = i == j ? f[j] : x;
+      const float r = (float)fmin(fmax(rint(__ddiv_rn(__dsub_rn((double)x, (double)minimum), (double)scale)), 0.0), 15.0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = i == j ? r : c[j];
+    }
+  }
+  uint32_t half[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float v = __fmaf_rn(c[4 * k + 3], 16.0f, c[4 * k + 2]);
+    v = __fmaf_rn(v, 16.0f, c[4 * k + 1]);
+    v = __fmaf_rn(v, 16.0f, c[4 * k]);
+    half[k] = __float_as_uint(__fadd_rn(v, 8388608.0f));
+  }
+  return __byte_perm(half[0], half[1], 0x5410);
 }
 
-template <int L, bool READ>
+template <int TYPE, int L, bool READ>
 __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const Kv4Pool p, const Kv4RowsDev r, int chunks,
                                                                uint32_t* status) {
   pdl_enter();
@@ -126,90 +192,68 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const Kv4Pool p, 
   }
   const int t0 = chunk * kRowTokens, nt = min(kRowTokens, count - t0);
   if (nt <= 0) return;
-  const int d = p.head_dim, lane = threadIdx.x % L, group = threadIdx.x / L;
-  constexpr int kGroups = kRowThreads / L;
-  const int rows = nt * p.kv_heads * 2, tokens = 1 << p.token_shift;
-  const int bytes = r.dtype == MC_F32 ? 4 : 2;
+  const int d = p.head_dim, lane = threadIdx.x % L, group = threadIdx.x / L, tokens = 1 << p.token_shift;
+  constexpr int kGroups = kRowThreads / L, kBytes = TYPE == MC_F32 ? 4 : 2;
   const bool active = lane * 8 < d;
+  const long long block_bytes = head_block(tokens, d);
+  const int32_t* table = p.table + (long long)b * p.per_seq;
   bool bad = false, bad_page = false;
-  for (int base = 0; base < rows; base += kGroups * kRowsPerPass) {
-    RowAt at[kRowsPerPass];
-    float f[kRowsPerPass][8];
-    uint32_t word[kRowsPerPass];
-    __half2 pair[kRowsPerPass];
-    bool live[kRowsPerPass];
+  for (int pair0 = 0; pair0 < 2 * p.kv_heads; pair0 += kGroups) {
+    const int h = (pair0 + group) >> 1, which = group & 1;
+    const bool mine = h < p.kv_heads && active;
+    const long long rs = (which ? r.v_rs : r.k_rs) * kBytes;
+    char* x0 = static_cast<char*>(which ? r.v : r.k) + (start + t0) * rs + (h * (which ? r.v_hs : r.k_hs) + lane * 8) * kBytes;
+    for (int t = 0; t < nt; t += kRowsInFlight) {
+      Eight<TYPE> x[kRowsInFlight];
+      uint32_t word[kRowsInFlight];
+      __half2 pair[kRowsInFlight];
+      uint8_t* block[kRowsInFlight];  // of the row's page and head; nullptr: no row
 #pragma unroll
-    for (int u = 0; u < kRowsPerPass; ++u) {
-      const int row = base + u * kGroups + group;
-      live[u] = row < rows;
-      if (live[u]) {
-        const int hw = row / nt, tok = t0 + row - hw * nt, h = hw >> 1, which = hw & 1;
-        const int pos = first + tok;
-        const long long page = p.table[(long long)b * p.per_seq + (pos >> p.token_shift)];
+      for (int u = 0; u < kRowsInFlight; ++u) {
+        block[u] = nullptr;
+        const int pos = first + t0 + t + u;
+        if (!mine || t + u >= nt) continue;
+        const long long page = table[pos >> p.token_shift];
         if (page < 0 || page >= p.n_pages) {
-          live[u] = false;
           bad_page = true;
-        } else {
-          uint8_t* block = p.pages + (page * p.kv_heads + h) * (long long)head_block(tokens, d);
-          const int slot = pos & (tokens - 1);
-          at[u].codes = block + (which * tokens + slot) * (d / 2) + lane * 4;
-          at[u].params = reinterpret_cast<__half2*>(block + tokens * d) + which * tokens + slot;
-          const long long off = which ? (start + tok) * r.v_rs + h * r.v_hs : (start + tok) * r.k_rs + h * r.k_hs;
-          at[u].x = static_cast<char*>(which ? r.v : r.k) + (off + lane * 8) * bytes;
+          continue;
         }
-      }
-      live[u] = live[u] && active;
-      if (live[u]) {
+        block[u] = p.pages + (page * p.kv_heads + h) * block_bytes;
+        const int slot = which * tokens + (pos & (tokens - 1));
         if (READ) {
-          word[u] = __ldcs(reinterpret_cast<const uint32_t*>(at[u].codes));
-          pair[u] = *at[u].params;
+          word[u] = __ldcs(reinterpret_cast<const uint32_t*>(block[u] + slot * (d / 2)) + lane);
+          pair[u] = reinterpret_cast<const __half2*>(block[u] + tokens * d)[slot];
         } else {
-          load_eight(at[u].x, r.dtype, f[u]);
+          x[u].load(x0 + (t + u) * rs);
         }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < kRowsPerPass; ++u) {
-      if (READ) {
-        if (!live[u]) continue;
-        const float scale = __low2float(pair[u]), minimum = __high2float(pair[u]);
+      for (int u = 0; u < kRowsInFlight; ++u) {
+        const int slot = which * tokens + ((first + t0 + t + u) & (tokens - 1));
+        float f[8];
+        if (READ) {
+          if (!block[u]) continue;
+          const float scale = __low2float(pair[u]), minimum = __high2float(pair[u]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          f[u][i] = __fmaf_rn(scale, (float)((word[u] >> (4 * i)) & 15), minimum);
-        store_eight(at[u].x, r.dtype, f[u]);
-      } else {
-        float lo = INFINITY, hi = -INFINITY;
-        bool finite = true;
-        if (live[u]) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            finite = finite && isfinite(f[u][i]);
-            lo = fminf(lo, f[u][i]);
-            hi = fmaxf(hi, f[u][i]);
-          }
-        }
-        // A row's lanes agree on whether it is finite: a lane that saw a NaN
-        // or an infinity makes the row's minimum -inf.
-        if (!finite) lo = -INFINITY;
-        lo = group_min<L>(lo);
-        hi = group_max<L>(hi);
-        __half min_h = __float2half_rn(lo);
-        __half scale_h = __float2half_rn(__fmul_rn(__fsub_rn(hi, __half2float(min_h)), 1.0f / 15.0f));
-        if (!live[u]) continue;
-        uint32_t w = 0;
-        if (__hisinf(min_h) || __hisinf(scale_h) || __hisnan(scale_h)) {
-          bad = true;
-          min_h = scale_h = __float2half_rn(0.0f);
+          for (int i = 0; i < 8; ++i) f[i] = __fmaf_rn(scale, (float)((word[u] >> (4 * i)) & 15), minimum);
+          store_eight<TYPE>(x0 + (t + u) * rs, f);
         } else {
-          const float minimum = __half2float(min_h), scale = __half2float(scale_h);
-          if (scale > 0.0f) {
-            const float inverse = __frcp_rn(scale);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w |= code_of(f[u][i], minimum, scale, inverse) << (4 * i);
+          float low, high;
+          row_range<TYPE, L>(x[u], block[u] != nullptr, &low, &high);
+          if (!block[u]) continue;
+          __half min_h = __float2half_rn(low);
+          __half scale_h = __float2half_rn(__fmul_rn(__fsub_rn(high, __half2float(min_h)), 1.0f / 15.0f));
+          uint32_t w = 0;
+          if (__hisinf(min_h) || __hisinf(scale_h) || __hisnan(scale_h)) {
+            bad = true;
+            min_h = scale_h = __float2half_rn(0.0f);
+          } else if (__half2float(scale_h) > 0.0f) {
+            x[u].values(f);
+            w = codes_of(f, __half2float(min_h), __half2float(scale_h));
           }
+          reinterpret_cast<uint32_t*>(block[u] + slot * (d / 2))[lane] = w;
+          if (lane == 0) reinterpret_cast<__half2*>(block[u] + tokens * d)[slot] = __halves2half2(scale_h, min_h);
         }
-        *reinterpret_cast<uint32_t*>(at[u].codes) = w;
-        if (lane == 0) *at[u].params = __halves2half2(scale_h, min_h);
       }
     }
   }
@@ -244,15 +288,17 @@ struct Kv4AttnParams {
   AttnSplit split;
   float scale;
   int row_tiles, warps_log2;  // column tiles per (sequence, head); log2 warps per unit
-  long long units;
+  uint32_t units;
   uint32_t* status;
 };
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnStages = 4;
+constexpr int kAttnStages = 2;
 constexpr int kTileKeys = 32;
 
 __host__ __device__ constexpr int stage_bytes(int d) { return kTileKeys * (d + 8); }
+// CTAs per SM that the registers are kept to.
+constexpr int attn_blocks(int nt) { return nt == 1 ? 4 : 3; }
 __host__ __device__ constexpr int attn_smem(int d) {
   return kAttnWarps * kAttnStages * (stage_bytes(d) + 16);
 }
@@ -288,7 +334,7 @@ __device__ __forceinline__ float half_exponent(uint32_t bits) {
 }
 
 template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_kernel(const Kv4AttnParams p) {
+__global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_kernel(const Kv4AttnParams p) {
   constexpr int kCols = SPLIT ? 4 : 8;  // queries of a column tile
   constexpr int kQ = kCols * NT;
   constexpr int kSteps = D / 16;        // k16 steps of a score, m16 tiles of the output
@@ -308,23 +354,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_kernel(const Kv4Attn
 
   const AttnRows& r = p.rows;
   const int wpu = 1 << p.warps_log2, sub = warp & (wpu - 1);
-  const long long unit = (long long)blockIdx.x * (kAttnWarps >> p.warps_log2) + (warp >> p.warps_log2);
+  const uint32_t unit = blockIdx.x * (kAttnWarps >> p.warps_log2) + (warp >> p.warps_log2);
   const int split = blockIdx.y;
   bool live = unit < p.units;
   int b = 0, head = 0, tile = 0;
   if (live) {
-    const long long bh = unit / p.row_tiles;
+    const uint32_t bh = unit / (uint32_t)p.row_tiles;
     tile = (int)(unit - bh * p.row_tiles);
-    b = (int)(bh / r.kv_heads);
-    head = (int)(bh - (long long)b * r.kv_heads);
+    b = (int)(bh / (uint32_t)r.kv_heads);
+    head = (int)(bh - (uint32_t)b * r.kv_heads);
   }
   AttnSeq seq = {0, 0, 0, 0, false};
   if (live) seq = attn_seq(r, b, p.status, head == 0 && tile == 0 && split == 0 && sub == 0 && lane == 0);
   const int n_rows = seq.nq * r.group, row0 = tile * kQ;
   live = live && row0 < n_rows;
   // The keys that the unit's last query sees, and this warp's tiles of them.
-  const int pos_last = live ? min(seq.nq - 1, (row0 + kQ - 1) / r.group) : 0;
-  const int pos_first = live ? row0 / r.group : 0;
+  const int pos_last = live ? min(seq.nq - 1, (int)((uint32_t)(row0 + kQ - 1) / (uint32_t)r.group)) : 0;
+  const int pos_first = live ? (int)((uint32_t)row0 / (uint32_t)r.group) : 0;
   const int keys = live ? max(0, r.causal ? seq.nk - (seq.nq - 1 - pos_last) : seq.nk) : 0;
   const int keys_all = live ? max(0, r.causal ? seq.nk - (seq.nq - 1 - pos_first) : seq.nk) : 0;  // seen by every query
   const int splits_here = live ? max(1, ((seq.nk + kTileKeys - 1) / kTileKeys + p.split.chunk - 1) / p.split.chunk) : 0;
@@ -343,7 +389,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_kernel(const Kv4Attn
   for (int n = 0; n < NT; ++n) {
     const int row = row0 + n * kCols + col;
     const bool there = live && row < n_rows;
-    const int pos = there ? row / r.group : 0, h = head * r.group + (there ? row - pos * r.group : 0);
+    const int pos = there ? (int)((uint32_t)row / (uint32_t)r.group) : 0, h = head * r.group + (there ? row - pos * r.group : 0);
     const char* src = static_cast<const char*>(r.q) +
                       ((long long)(seq.q0 + pos) * r.q_row_stride + (long long)h * r.q_head_stride) *
                           (r.dtype == MC_F32 ? 4 : 2);
@@ -409,7 +455,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_kernel(const Kv4Attn
   const int32_t* table = p.pool.table + (long long)b * p.pool.per_seq;
   int ids = -1, ids_at = -1000;
   auto issue = [&](int tl) {
-    const int s = (tl - begin) & (kAttnStages - 1), blk = tl * blocks;
+    const int s = (tl - begin) % kAttnStages, blk = tl * blocks;
     if (ids_at < 0 || blk + blocks > ids_at + 32) {
       ids_at = blk;
       ids = blk + lane < n_blocks ? table[blk + lane] : -1;
@@ -454,11 +500,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_kernel(const Kv4Attn
 
   bool broken = false;
   for (int tl = begin; tl < end; ++tl) {
-    const int s = (tl - begin) & (kAttnStages - 1);
+    const int s = (tl - begin) % kAttnStages;
     if (!mbar_wait(&bars[s], ((tl - begin) / kAttnStages) & 1, p.status)) {
       // Let the copies of the other stages land before the block leaves.
       for (int k = tl + 1; k < min(end, tl + kAttnStages); ++k)
-        mbar_wait(&bars[(k - begin) & (kAttnStages - 1)], ((k - begin) / kAttnStages) & 1, p.status);
+        mbar_wait(&bars[(k - begin) % kAttnStages], ((k - begin) / kAttnStages) & 1, p.status);
       broken = true;
       break;
     }
@@ -677,7 +723,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_kernel(const Kv4Attn
   if (join) __syncthreads();  // the rings of a unit's warps become their results
   float* own_out = reinterpret_cast<float*>(ring);
   float* own_lse = own_out + kQ * D;
-  const long long slot0 = unit * kQ;
+  const long long slot0 = (long long)unit * kQ;
   const bool direct = splits_here <= 1;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -692,6 +738,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_kernel(const Kv4Attn
       inv[j] = sum_p[n][j] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum_p[n][j]);
       zero[j] = sum_m[n][j];
       lse2[j] = sum_p[n][j] == 0.0f ? -INFINITY : __fadd_rn(__fsub_rn(top[n][j], 10.0f), log2f(sum_p[n][j]));
+    }
+    long long at[2];  // where the lane's columns go: their output row, or their slot
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = min(row0 + n * kCols + 2 * t + j, max(n_rows - 1, 0));
+      const int pos = (int)((uint32_t)row / (uint32_t)r.group), h = head * r.group + row - pos * r.group;
+      at[j] = direct ? (long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride
+                     : ((slot0 + n * kCols + 2 * t + j) * p.split.splits + split) * D;
     }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -720,13 +774,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_kernel(const Kv4Attn
         if (join) {
           *reinterpret_cast<float2*>(own_out + q * D + 2 * byte) = make_float2(even, odd);
         } else if (direct) {
-          const int pos = (row0 + q) / r.group, h = head * r.group + (row0 + q) - pos * r.group;
-          store2(r.out,
-                 (long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride + 2 * byte, r.dtype,
-                 even, odd);
+          store2(r.out, at[j] + 2 * byte, r.dtype, even, odd);
         } else {
-          *reinterpret_cast<float2*>(p.split.out + ((slot0 + q) * p.split.splits + split) * D + 2 * byte) =
-              make_float2(even, odd);
+          *reinterpret_cast<float2*>(p.split.out + at[j] + 2 * byte) = make_float2(even, odd);
         }
       }
     }
@@ -920,10 +970,19 @@ Kv4Pool pool_of(const mc_kv4_cache* c) {
   return p;
 }
 
-template <int L, bool READ>
+template <int TYPE, int L, bool READ>
 cudaError_t launch_rows(const Kv4Pool& p, const Kv4RowsDev& r, long long grid, int chunks, uint32_t* status,
                         cudaStream_t s) {
-  return launch_pdl(kv4_rows_kernel<L, READ>, dim3((unsigned)grid), dim3(kRowThreads), 0, s, p, r, chunks, status);
+  return launch_pdl(kv4_rows_kernel<TYPE, L, READ>, dim3((unsigned)grid), dim3(kRowThreads), 0, s, p, r, chunks, status);
+}
+template <int TYPE, bool READ>
+cudaError_t launch_rows_l(const Kv4Pool& p, const Kv4RowsDev& r, long long grid, int chunks, uint32_t* status,
+                          cudaStream_t s) {
+  const int lanes = p.head_dim / 8;
+  return lanes <= 2   ? launch_rows<TYPE, 2, READ>(p, r, grid, chunks, status, s)
+         : lanes <= 4 ? launch_rows<TYPE, 4, READ>(p, r, grid, chunks, status, s)
+         : lanes <= 8 ? launch_rows<TYPE, 8, READ>(p, r, grid, chunks, status, s)
+                      : launch_rows<TYPE, 16, READ>(p, r, grid, chunks, status, s);
 }
 
 template <bool READ>
@@ -946,14 +1005,12 @@ mc_status kv4_rows(const mc_kv4_cache* c, const mc_kv4_rows* a, void* stream) {
   uint32_t* status = op_status_word();
   if (!status) return MC_CUDA;
   const Kv4Pool pool = pool_of(c);
-  const Kv4RowsDev r = {a->k,           a->v,           a->start,       a->count,        a->first,       a->rows,
-                        a->k_row_stride, a->k_head_stride, a->v_row_stride, a->v_head_stride, a->dtype, a->max_count};
+  const Kv4RowsDev r = {a->k,           a->v,           a->start,       a->count,        a->first,      a->rows,
+                        a->k_row_stride, a->k_head_stride, a->v_row_stride, a->v_head_stride, a->max_count};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int lanes = c->head_dim / 8;
-  const cudaError_t e = lanes <= 2   ? launch_rows<2, READ>(pool, r, grid, (int)chunks, status, s)
-                        : lanes <= 4 ? launch_rows<4, READ>(pool, r, grid, (int)chunks, status, s)
-                        : lanes <= 8 ? launch_rows<8, READ>(pool, r, grid, (int)chunks, status, s)
-                                     : launch_rows<16, READ>(pool, r, grid, (int)chunks, status, s);
+  const cudaError_t e = a->dtype == MC_F32   ? launch_rows_l<MC_F32, READ>(pool, r, grid, (int)chunks, status, s)
+                        : a->dtype == MC_F16 ? launch_rows_l<MC_F16, READ>(pool, r, grid, (int)chunks, status, s)
+                                             : launch_rows_l<MC_BF16, READ>(pool, r, grid, (int)chunks, status, s);
   return e == cudaSuccess ? MC_OK : MC_CUDA;
 }
 
@@ -1038,7 +1095,7 @@ extern "C" mc_status mc_kv4_attention(const mc_kv4_cache* c, const mc_kv4_attent
   p.scale = a->scale;
   p.row_tiles = plan.row_tiles;
   p.warps_log2 = plan.warps_log2;
-  p.units = plan.units;
+  p.units = (uint32_t)plan.units;
   p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaErrorInvalidValue;
