@@ -80,10 +80,12 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = high + low: the upper 11 bits of the mantissa, and the rest.
-__device__ __forceinline__ uint32_t tf32_high(float x) { return __float_as_uint(x) & 0xFFFFE000u; }
+// x = high + low: x rounded to 11 bits, and the rest.  (Cut off instead of
+// rounded, the rests are all of one sign, and so are the errors of the 11 bits
+// that are left of them: outputs 8e-7 off instead of 5e-7.)
+__device__ __forceinline__ uint32_t tf32_high(float x) { return (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u; }
 __device__ __forceinline__ uint32_t tf32_low(float x) {
-  return __float_as_uint(__fsub_rn(x, __uint_as_float(__float_as_uint(x) & 0xFFFFE000u)));
+  return __float_as_uint(__fsub_rn(x, __uint_as_float(tf32_high(x))));
 }
 __device__ __forceinline__ void mma_split(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0,
                                           float b1) {
@@ -108,8 +110,8 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
   pdl_enter();
 
   const AttnRows& r = p.rows;
-  const long long unit = blockIdx.x, bh = unit / p.row_tiles;
-  const int tile = (int)(unit - bh * p.row_tiles), b = (int)(bh / r.kv_heads), head = (int)(bh - (long long)b * r.kv_heads);
+  const uint32_t unit = blockIdx.x, bh = unit / (uint32_t)p.row_tiles;
+  const int tile = (int)(unit - bh * p.row_tiles), b = (int)(bh / (uint32_t)r.kv_heads), head = (int)(bh - (uint32_t)b * r.kv_heads);
   const int split = blockIdx.y;
   const AttnSeq seq = attn_seq(r, b, p.status, head == 0 && tile == 0 && split == 0 && tid == 0);
   const int n_rows = seq.nq * r.group, row0 = tile * kRows;
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
   for (int h = 0; h < 2; ++h) {
     const int row = own + g + 8 * h;
     there[h] = row < n_rows;
-    const int pos = there[h] ? row / r.group : 0, qh = head * r.group + (there[h] ? row - pos * r.group : 0);
+    const int pos = there[h] ? (int)((uint32_t)row / (uint32_t)r.group) : 0, qh = head * r.group + (there[h] ? row - pos * r.group : 0);
     src[h] = static_cast<const T*>(r.q) + (long long)(seq.q0 + pos) * r.q_row_stride + (long long)qh * r.q_head_stride;
   }
   const bool busy = own < n_rows;
@@ -203,6 +205,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
       const int s = tl & (kStages - 1);
       const T* ks = ring + s * 2 * kElems + kg * kOwn * kPitch;
       const T* vs = ks + kElems;
+      const int keys = seq.nk - tl * kKeys - kg * kOwn;  // of this warp's; n-tiles past them are left out
       float x[kNT][4];
 #pragma unroll
       for (int j = 0; j < kNT; ++j)
@@ -222,6 +225,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
           }
 #pragma unroll
           for (int j = 0; j < kNT; ++j) {
+            if (8 * j >= keys) break;
             const float2 kv = *reinterpret_cast<const float2*>(ks + (8 * j + (g >> 1) + 4 * (g & 1)) * kPitch + 8 * c + 2 * t);
             mma_split(x[j], ah, al, kv.x, kv.y);
           }
@@ -231,6 +235,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
         for (int c = 0; c < D / 16; ++c)
 #pragma unroll
           for (int j = 0; j < kNT; j += 2) {
+            if (8 * j >= keys) break;
             uint32_t kb[4];
             ldsm4(kb, ks + (8 * j + (lane & 7) + (lane >> 4) * 8) * kPitch + 16 * c + ((lane >> 3) & 1) * 8);
             if constexpr (sizeof(T) == 2) {
@@ -296,6 +301,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
       if constexpr (kF32) {
 #pragma unroll
         for (int j = 0; j < kNT; ++j) {
+          if (8 * j >= keys) break;
           uint32_t ah[4], al[4];
           // k = t: column 2 t (key t); k = t + 4: column 2 t + 1 (key t + 4)
           ah[0] = tf32_high(x[j][0]); ah[1] = tf32_high(x[j][2]); ah[2] = tf32_high(x[j][1]); ah[3] = tf32_high(x[j][3]);
@@ -312,6 +318,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
       } else {
 #pragma unroll
         for (int j = 0; j < kNT; j += 2) {
+          if (8 * j >= keys) break;
           uint32_t a[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -345,31 +352,38 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
     inv[h] = sum[h] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum[h]);
     lse2[h] = sum[h] == 0.0f ? -INFINITY : __fadd_rn(__fsub_rn(top[h], kShift), log2f(sum[h]));
   }
-  const long long slot0 = unit * kRows;
+  const long long slot0 = (long long)unit * kRows;
   const bool direct = parts <= 1;
-  auto emit = [&](int row, int ch, float a, float e) {  // row of the unit
-    if (direct) {
-      const int pos = (row0 + row) / r.group, h = head * r.group + (row0 + row) - pos * r.group;
-      store2(r.out, (long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride + ch, r.dtype, a, e);
-    } else {
-      *reinterpret_cast<float2*>(p.split.out + ((slot0 + row) * p.split.splits + split) * D + ch) = make_float2(a, e);
-    }
+  struct Place {
+    long long out, lse;
   };
-  auto emit_lse = [&](int row, float l) {
-    if (!direct) {
-      p.split.lse[(slot0 + row) * p.split.splits + split] = l;
-    } else if (r.lse) {
-      const int pos = (row0 + row) / r.group, h = head * r.group + (row0 + row) - pos * r.group;
-      r.lse[(long long)(seq.q0 + pos) * r.kv_heads * r.group + h] = __fmul_rn(l, kLn2);
-    }
+  auto place_of = [&](int row) {  // of the unit
+    if (!direct) return Place{((slot0 + row) * p.split.splits + split) * D, (slot0 + row) * p.split.splits + split};
+    const int pos = (int)((uint32_t)(row0 + row) / (uint32_t)r.group), h = head * r.group + (row0 + row) - pos * r.group;
+    return Place{(long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride,
+                 (long long)(seq.q0 + pos) * r.kv_heads * r.group + h};
+  };
+  auto emit = [&](const Place& to, int ch, float a, float e) {
+    if (direct)
+      store2(r.out, to.out + ch, r.dtype, a, e);
+    else
+      *reinterpret_cast<float2*>(p.split.out + to.out + ch) = make_float2(a, e);
+  };
+  auto emit_lse = [&](const Place& to, float l) {
+    if (!direct)
+      p.split.lse[to.lse] = l;
+    else if (r.lse)
+      r.lse[to.lse] = __fmul_rn(l, kLn2);
   };
   float* part = reinterpret_cast<float*>(smem) + (kg * WR + wr) * 16 * (D + 1);
 #pragma unroll
-  for (int i = 0; i < kOut; i += (kF32 ? 2 : 1))
+  for (int h = 0; h < 2; ++h) {
+    const int row = wr * 16 + g + 8 * h;
+    if (row0 + row >= n_rows) continue;
+    Place to = {};
+    if (kGroups == 1) to = place_of(row);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = wr * 16 + g + 8 * h;
-      if (row0 + row >= n_rows) continue;
+    for (int i = 0; i < kOut; i += (kF32 ? 2 : 1)) {
       if constexpr (kF32) {
         // tiles i, i + 1: channels 8 i + 4 t + {0, 1} of column 2 t, + {2, 3} of column 2 t + 1
 #pragma unroll
@@ -377,7 +391,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
           const float a = __fmul_rn(acc[i][2 * h + e], inv[h]), c = __fmul_rn(acc[i + 1][2 * h + e], inv[h]);
           const int ch = 8 * i + 4 * t + 2 * e;
           if (kGroups == 1) {
-            emit(row, ch, a, c);
+            emit(to, ch, a, c);
           } else {
             part[(g + 8 * h) * D + ch] = a;
             part[(g + 8 * h) * D + ch + 1] = c;
@@ -387,20 +401,16 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
         const float a = __fmul_rn(acc[i][2 * h], inv[h]), c = __fmul_rn(acc[i][2 * h + 1], inv[h]);
         const int ch = 8 * i + 2 * t;
         if (kGroups == 1) {
-          emit(row, ch, a, c);
+          emit(to, ch, a, c);
         } else {
           part[(g + 8 * h) * D + ch] = a;
           part[(g + 8 * h) * D + ch + 1] = c;
         }
       }
     }
-  if (t == 0) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = wr * 16 + g + 8 * h;
-      if (row0 + row >= n_rows) continue;
+    if (t == 0) {
       if (kGroups == 1)
-        emit_lse(row, lse2[h]);
+        emit_lse(to, lse2[h]);
       else
         part[16 * D + g + 8 * h] = lse2[h];
     }
@@ -423,6 +433,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
       total = __fadd_rn(total, w[k]);
     }
     const float scale = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+    const Place to = place_of(row);
     for (int ch = 2 * lane; ch < D; ch += 64) {
       float a = 0.0f, e = 0.0f;
 #pragma unroll
@@ -431,9 +442,9 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
           a = __fmaf_rn(w[k], of[k * kStep + (row % 16) * D + ch], a);
           e = __fmaf_rn(w[k], of[k * kStep + (row % 16) * D + ch + 1], e);
         }
-      emit(row, ch, __fmul_rn(a, scale), __fmul_rn(e, scale));
+      emit(to, ch, __fmul_rn(a, scale), __fmul_rn(e, scale));
     }
-    if (lane == 0) emit_lse(row, total == 0.0f ? -INFINITY : __fadd_rn(best, log2f(total)));
+    if (lane == 0) emit_lse(to, total == 0.0f ? -INFINITY : __fadd_rn(best, log2f(total)));
   }
 }
 
