@@ -1,0 +1,116 @@
+"""The decode-step operators together, as a decoder that samples several
+translations of each source uses them: every step appends the new token's keys
+and values to the 4-bit cache, attends over it, attends to the encoder's states
+(which the translations of one source share) and draws the next token.
+
+Every operator's result is compared with the 64-bit form of its definition on
+the inputs that it was given, so no error adds up; tolerances as in each
+operator's own tests.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from marian_cuda import _lib as L  # noqa: E402
+from test_cross_attention import arguments as cross_arguments, attend as cross_attend  # noqa: E402
+from test_kv4 import Cache, attend as kv_attend, ints, quantize, rows_struct, score_error, status_bits  # noqa: E402
+from test_sample import reference as sample_reference  # noqa: E402
+
+HEADS, DIM, VOCAB, STEPS = 4, 48, 977, 21
+D = HEADS * DIM
+
+
+def f64(x):
+    return x.float().cpu().numpy().astype(np.float64)
+
+
+class Decoder:
+    """One attention layer of random weights in f32, over the library's operators."""
+
+    def __init__(self, src_len, copies, seed):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+        self.embed = rnd(VOCAB, D)
+        self.w = {n: rnd(D, D) / D ** 0.5 for n in ("q", "k", "v", "o", "cq")}
+        self.out = rnd(D, VOCAB) * 3 / D ** 0.5
+        self.batch = len(src_len) * copies
+        src = int(np.sum(src_len))
+        self.enc_k, self.enc_v = rnd(src, HEADS, DIM), rnd(src, HEADS, DIM)
+        start = np.cumsum(src_len) - src_len
+        self.k_start, self.k_len = np.repeat(start, copies), np.repeat(src_len, copies)
+        self.cache = Cache(self.batch, -(-STEPS // 8), 8, HEADS, DIM, fill=0xFF)
+        self.uniform = torch.rand(STEPS, self.batch, generator=g, device="cuda")
+        self.temperature = torch.linspace(0.0, 1.2, self.batch, device="cuda")
+        self.one = ints(np.ones(self.batch))
+        self.rows = ints(np.arange(self.batch))
+        self.source = [ints(self.k_start), ints(self.k_len)]
+
+    def step(self, t, tokens, stream):
+        lib, b = L.load(), self.batch
+        x = self.embed[tokens.long()]
+        q, k, v = ((x @ self.w[n]).view(b, HEADS, DIM) for n in ("q", "k", "v"))
+        cache = self.cache.struct()
+        new = rows_struct(k, v, np.arange(b), np.ones(b), np.full(b, t), 1, L.MC_F32)
+        assert lib.mc_kv4_append(C.byref(cache), C.byref(new), stream) == L.MC_OK
+        held, self_out = ints(np.full(b, t + 1)), torch.empty_like(q)
+        a = L.Kv4AttentionArgs(q=q.data_ptr(), out=self_out.data_ptr(), q_start=self.rows.data_ptr(),
+                               q_len=self.one.data_ptr(), kv_len=held.data_ptr(), q_rows=b, q_row_stride=D,
+                               q_head_stride=DIM, out_row_stride=D, out_head_stride=DIM, dtype=L.MC_F32, heads=HEADS,
+                               max_q_len=1, max_kv_len=STEPS, causal=1, scale=DIM ** -0.5)
+        assert lib.mc_kv4_attention_workspace(C.byref(cache), C.byref(a)) == 0
+        assert lib.mc_kv4_attention(C.byref(cache), C.byref(a), stream) == L.MC_OK
+        y = x + self_out.view(b, D) @ self.w["o"]
+        cq = (y @ self.w["cq"]).view(b, HEADS, DIM).contiguous()
+        cross_out = torch.empty_like(cq)
+        ca, _ = cross_arguments(cq, self.enc_k, self.enc_v, cross_out, None, [self.rows, self.one] + self.source, None,
+                                "f32", DIM ** -0.5, 1, int(self.k_len.max()))
+        assert lib.mc_cross_attention(C.byref(ca), stream) == L.MC_OK
+        logits = (y + cross_out.view(b, D)) @ self.out
+        nxt, probs = torch.empty(b, dtype=torch.int32, device="cuda"), torch.empty(b, device="cuda")
+        top_k, top_p = ints(np.full(b, 40)), torch.full((b,), 0.95, device="cuda")
+        s = L.SampleArgs(logits=logits.data_ptr(), temperature=self.temperature.data_ptr(), top_k=top_k.data_ptr(),
+                         top_p=top_p.data_ptr(), uniform=self.uniform[t].data_ptr(), tokens=nxt.data_ptr(),
+                         probs=probs.data_ptr(), row_stride=VOCAB, dtype=L.MC_F32, rows=b, vocab=VOCAB)
+        assert lib.mc_sample(C.byref(s), stream) == L.MC_OK
+        torch.cuda.current_stream().synchronize()
+        return dict(q=q, k=k, v=v, self_out=self_out, cq=cq, cross_out=cross_out, logits=logits, tokens=nxt, probs=probs)
+
+
+@pytest.mark.parametrize("src_len,copies", [([17], 1), ([5, 40, 1], 3), ([64, 130], 40)])
+def test_sampled_translations_step_by_step(src_len, copies):
+    dec = Decoder(src_len, copies, seed=len(src_len) + copies)
+    scale = DIM ** -0.5
+    tokens = torch.arange(dec.batch, dtype=torch.int32, device="cuda") % VOCAB
+    held = [[], []]
+    enc_k, enc_v = f64(dec.enc_k), f64(dec.enc_v)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for t in range(STEPS):
+            r = dec.step(t, tokens, stream.cuda_stream)
+            for h, n in zip(held, ("k", "v")):
+                c, s, m = quantize(f64(r[n]))
+                h.append(m.astype(np.float64)[..., None] + s.astype(np.float64)[..., None] * c)
+            q, cq, got, cross = (f64(r[n]) for n in ("q", "cq", "self_out", "cross_out"))
+            for i in range(dec.batch):
+                k, v = (np.stack([row[i] for row in h]) for h in held)
+                want, _ = kv_attend(q[i:i + 1], k, v, scale, lambda _: t + 1)
+                tol = (2.0 ** -18 + 2 * score_error(q[i:i + 1], k, scale)) * np.abs(v).max()
+                np.testing.assert_allclose(got[i:i + 1], want, rtol=0, atol=tol)
+                at = slice(dec.k_start[i], dec.k_start[i] + dec.k_len[i])
+                want, _ = cross_attend(cq[i:i + 1], enc_k[at], enc_v[at], scale, np.ones(dec.k_len[i], bool))
+                dx = 2.0 ** -20 * scale * np.abs(cq[i]).sum(-1).max() * np.abs(enc_k[at]).max()
+                np.testing.assert_allclose(cross[i:i + 1], want, rtol=0, atol=(2.0 ** -18 + 2 * dx) * np.abs(enc_v[at]).max())
+            logits, u, temperature = f64(r["logits"]), f64(dec.uniform[t]), f64(dec.temperature)
+            for i in range(dec.batch):
+                token, prob = sample_reference(logits[i], temperature[i], 40, float(np.float32(0.95)), 0.0, u[i])
+                assert int(r["tokens"][i]) == token and float(r["probs"][i]) == pytest.approx(prob, rel=2.0 ** -20)
+            tokens = r["tokens"]
+    assert status_bits() == 0
+    if copies > 1:   # the copies of a source draw different translations
+        assert len({int(x) for x in tokens}) > 1
