@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
 struct CrossPlan {
   bool long_tiles;
   int tile_rows, row_tiles, splits, chunk, tile_keys;
-  long long units;
+  long long units, first;
   uint64_t slots, bytes;
 };
 
@@ -483,13 +483,24 @@ CrossPlan cross_plan(const mc_cross_attention_args* a, bool long_tiles) {
   // Ranges of keys for units too few to fill the GPU (one long CTA or three
   // small ones per SM), each of four tiles at least.
   const int tiles = (int)(((int64_t)a->max_k_len + plan.tile_keys - 1) / plan.tile_keys);
-  long long splits = plan.units > 0 ? kSms * (long_tiles ? 1 : 3) / plan.units : 1;
+  // Long CTAs take one SM each, in waves; the last wave's units are cut too
+  // where they are half of one or less (512 units of 64 tiles: four waves of
+  // which the last is 68 units, 605 us; three and a half, 570 us).
+  plan.first = 0;
+  long long cut = plan.units;
+  if (long_tiles && plan.units > kSms) {
+    cut = plan.units % kSms;
+    if (cut > kSms / 2) cut = 0;
+    plan.first = plan.units - cut;
+  }
+  long long splits = cut > 0 ? kSms * (long_tiles ? 1 : 3) / cut : 1;
   if (splits > tiles / 4) splits = tiles / 4;
   if (splits > 256) splits = 256;
   if (splits < 1) splits = 1;
   plan.chunk = tiles > 0 ? (int)((tiles + splits - 1) / splits) : 1;
   plan.splits = tiles > 0 ? (tiles + plan.chunk - 1) / plan.chunk : 1;
-  plan.slots = (uint64_t)plan.units * plan.tile_rows;
+  if (plan.splits == 1) plan.first = 0;
+  plan.slots = (uint64_t)(plan.units - plan.first) * plan.tile_rows;
   plan.bytes = attn_split_bytes(plan.slots, plan.splits, a->head_dim);
   return plan;
 }
@@ -534,6 +545,7 @@ cudaError_t launch_small_d(const CrossParams& p, const CrossPlan& plan, cudaStre
 cudaError_t launch_cross(CrossParams p, const CrossPlan& plan, void* workspace, cudaStream_t s) {
   p.split.splits = plan.splits;
   p.split.chunk = plan.chunk;
+  p.split.first = (uint32_t)plan.first;
   p.row_tiles = plan.row_tiles;
   if (plan.splits > 1) {
     p.split.out = static_cast<float*>(workspace);

@@ -217,15 +217,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_enter();
 
   const AttnRows& r = p.rows;
-  const long long unit = blockIdx.x, bh = unit / p.row_tiles;
-  const int tile = (int)(unit - bh * p.row_tiles), b = (int)(bh / r.kv_heads), head = (int)(bh - (long long)b * r.kv_heads);
-  const int split = blockIdx.y;
+  // Whole units first, then the cut ones, range by range.
+  const uint32_t cut_block = blockIdx.x < p.split.first ? 0 : blockIdx.x - p.split.first;
+  const bool whole = blockIdx.x < p.split.first;
+  const uint32_t nth = cut_block / (uint32_t)p.split.splits, unit = whole ? blockIdx.x : p.split.first + nth;
+  const uint32_t bh = unit / (uint32_t)p.row_tiles;
+  const int tile = (int)(unit - bh * p.row_tiles), b = (int)(bh / (uint32_t)r.kv_heads), head = (int)(bh - (uint32_t)b * r.kv_heads);
+  const int split = whole ? 0 : (int)(cut_block - nth * p.split.splits);
   const AttnSeq seq = attn_seq(r, b, p.status, head == 0 && tile == 0 && split == 0 && threadIdx.x == 0);
   const int n_rows = seq.nq * r.group, row0 = tile * kLongRows;
   const int n_tiles = (seq.nk + kLongKeys - 1) / kLongKeys;
-  const int parts = max(1, (n_tiles + p.split.chunk - 1) / p.split.chunk);
+  const int chunk = whole ? max(n_tiles, 1) : p.split.chunk, parts = max(1, (n_tiles + chunk - 1) / chunk);
   const bool live = seq.ok && row0 < n_rows && split < parts;
-  const int begin = split * p.split.chunk, end = live ? min(n_tiles, begin + p.split.chunk) : begin;
+  const int begin = split * chunk, end = live ? min(n_tiles, begin + chunk) : begin;
   const int steps = end - begin;
   const int row_tiles = row0 + 128 < n_rows ? 2 : 1;
   const int spare = steps > 0 ? max(0, end * kLongKeys - seq.nk) : 0;  // keys of the last tile behind the sequence
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
     const float lse2 = sum == 0.0f ? -INFINITY : __fadd_rn(__fmul_rn(top, factor), log2f(sum));
     const bool direct = parts <= 1;
-    const long long slot = (unit * kLongRows + 128 * i + row_in) * p.split.splits + split;
+    const long long slot = ((long long)nth * kLongRows + 128 * i + row_in) * p.split.splits + split;
     if (ok) tc_fence_after();
     if (__any_sync(kFull, written && there)) {
 #pragma unroll
@@ -530,7 +534,7 @@ cudaError_t launch_long(const CrossParams& p, long long units, const CUtensorMap
   static uint64_t done = 0;
   cudaError_t e = allow_smem(cross_long_kernel<D, BF16>, long_smem(D), &done);
   if (e != cudaSuccess) return e;
-  return launch_pdl(cross_long_kernel<D, BF16>, dim3((unsigned)units, p.split.splits), dim3(kThreads), long_smem(D), s, p, k, v);
+  return launch_pdl(cross_long_kernel<D, BF16>, dim3((unsigned)(p.split.first + (units - p.split.first) * p.split.splits)), dim3(kThreads), long_smem(D), s, p, k, v);
 }
 
 template <int D>

@@ -116,11 +116,13 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnRows& r, int b, uint32_t* 
 // the keys of a unit are cut into ranges of `chunk` tiles, one CTA each;
 // every range writes its normalized rows and their log2-sum-exp2, and
 // attn_join averages them.  A sequence whose keys fit one range writes its
-// rows at once, and attn_join leaves it alone.
+// rows at once, and attn_join leaves it alone.  Units before `first` are
+// whole: a launch may cut its last ones only.
 struct AttnSplit {
-  float* out;  // [units * rows][splits][head_dim]
-  float* lse;  // [units * rows][splits], base 2
+  float* out;  // [(units - first) * rows][splits][head_dim]
+  float* lse;  // [(units - first) * rows][splits], base 2
   int splits, chunk;
+  uint32_t first;
 };
 
 cudaError_t launch_attn_join(const AttnRows& r, const AttnSplit& s, int tile_keys, int unit_rows, int row_tiles,

@@ -850,9 +850,9 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnRows r, const 
   const long long slot = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (slot >= slots) return;
-  const long long unit = slot / unit_rows, bh = unit / row_tiles;
-  const int q = (int)(slot - unit * unit_rows) + (int)(unit - bh * row_tiles) * unit_rows;
-  const int b = (int)(bh / r.kv_heads), head = (int)(bh - (long long)b * r.kv_heads);
+  const uint32_t nth = (uint32_t)(slot / unit_rows), unit = s.first + nth, bh = unit / (uint32_t)row_tiles;
+  const int q = (int)(slot - (long long)nth * unit_rows) + (int)(unit - bh * row_tiles) * unit_rows;
+  const int b = (int)(bh / (uint32_t)r.kv_heads), head = (int)(bh - (uint32_t)b * r.kv_heads);
   const AttnSeq seq = attn_seq(r, b, nullptr, false);
   if (!seq.ok || q >= seq.nq * r.group) return;
   const int parts = ((seq.nk + tile_keys - 1) / tile_keys + s.chunk - 1) / s.chunk;
@@ -1018,7 +1018,7 @@ mc_status kv4_rows(const mc_kv4_cache* c, const mc_kv4_rows* a, void* stream) {
 
 cudaError_t launch_attn_join(const AttnRows& r, const AttnSplit& s, int tile_keys, int unit_rows, int row_tiles,
                              cudaStream_t stream) {
-  const long long slots = (long long)r.batch * r.kv_heads * row_tiles * unit_rows;
+  const long long slots = ((long long)r.batch * r.kv_heads * row_tiles - s.first) * unit_rows;
   return launch_pdl(attn_join_kernel, dim3((unsigned)((slots + 3) / 4)), dim3(128), 0, stream, r, s, tile_keys,
                     unit_rows, row_tiles, slots);
 }

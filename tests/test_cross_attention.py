@@ -370,3 +370,16 @@ def test_rows_past_2_gib():
         k[rows - n:] = kv.cuda()
         out, lse, _ = run(q.cuda(), k, k, [0], [q_len], [rows - n], [n], "bf16", d ** -0.5)
         compare(q, kv, kv, out, lse, [0], [q_len], [0], [n], "bf16", d ** -0.5)
+
+
+@gpu
+@pytest.mark.parametrize("h,hk,cut", [(16, 8, False), (6, 3, True)])
+def test_long_sequences_in_several_waves(h, hk, cut):
+    # units of 256 rows, 13 sequences of up to 1,024 rows a head: 416 (the last wave more than half
+    # full) or 156, of which the keys of the last 8 are cut into ranges; among them a sequence without
+    # keys, one with few, one with no queries
+    rng = np.random.default_rng(6)
+    need = check(rng, [512] * 9 + [300, 0, 257, 256], [1100] * 8 + [0, 900, 1100, 130, 1100], h, hk, 32, "bf16")
+    assert (need > 0) == cut
+    need = check(rng, [512] * 9 + [300, 0, 256, 257], [1100] * 11 + [130, 0], h, hk, 32, "bf16")
+    assert (need > 0) == cut
