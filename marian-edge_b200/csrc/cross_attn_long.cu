@@ -10,7 +10,17 @@
 // 4-7 and 8-11 hold one query row per thread of tile 0 and 1: they read S_i,
 // keep the row's maximum and sum, and write the weights, rounded to the
 // type, over S_i.  O_i is only rescaled when a maximum grows by more than 8
-// (in powers of two): the weights stay below 2^8 and exact in their ratio.
+// (in powers of two): the weights stay below 2^8, and their sum is as stale.
+//
+// What bounds it: with M = N = 128 the tensor pipe, one issuing warp's round
+// through its barriers between the products of a step, and the exponentials
+// (16 a cycle) share the time.  Measured at 2 x 4,096 x 8,192, 16 heads of 128,
+// bf16 (329 us at the measured GEMM rate): MMAs without weights 514 us; a
+// quarter of the exponentials by a polynomial on the FMA pipe 4% slower; the
+// weights handed over by halves 2% slower; votes after the MMA warp's waits 3%
+// slower; K and V in stages of their own, and an arrival for every product,
+// 10% slower; a stage peeked at with try_wait, whose suspension takes some
+// hundred cycles, 20% slower.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -25,10 +35,6 @@ constexpr uint32_t kFull = 0xFFFFFFFFu;
 constexpr int kThreads = 384;
 constexpr int kTileBytes = 128 * 128;  // 128 rows of 64 channels
 constexpr float kGrowth = 8.0f;
-// Of the weights' exponentials, one pair in kPolyEvery is computed on the FMA
-// pipe: the special-function unit (16 a cycle) would take as long for a tile's
-// 16,384 as the tensor cores for both its products.
-constexpr int kPolyEvery = 4;
 
 constexpr int chunks_of(int d) { return (d + 63) / 64; }
 // Ring stages, each for the V tile of one step and the K tile of the next,
@@ -38,7 +44,7 @@ constexpr int long_smem(int d) { return (2 + 2 * stages_of(d)) * chunks_of(d) * 
 
 struct Barriers {
   uint64_t full[4], empty[4];
-  uint64_t k0_full, k0_done, q_ready, s_full[2], w_ready[2][2], o_done[2], v_clean;
+  uint64_t k0_full, k0_done, q_ready, s_full[2], w_ready[2], o_done[2], v_clean;
   uint32_t tmem, stop;
 };
 
@@ -53,13 +59,9 @@ __device__ __forceinline__ bool wait_for(Barriers* b, uint64_t* bar, uint32_t ph
   return false;
 }
 
-// The same for a whole warp, of which one lane polls, for waits that are
-// mostly long.  (The MMA warp's are short, and a lane's return costs more
-// there than the others' polling: 609 us against 580 at 2 x 4,096 x 8,192.)
+// The same for a whole warp, whose lanes agree on what came out.
 __device__ __forceinline__ bool warp_wait(Barriers* b, uint64_t* bar, uint32_t phase, uint32_t* status) {
-  bool ok = true;
-  if ((threadIdx.x & 31) == 0) ok = wait_for(b, bar, phase, status);
-  return __all_sync(kFull, ok);
+  return __all_sync(kFull, wait_for(b, bar, phase, status));
 }
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {
@@ -151,28 +153,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// 2^x of a pair on the FMA pipe: x = n + f, n whole (adding 1.5 * 2^23 rounds),
-// 2^f by the polynomial of degree 5 with the least largest relative error on
-// [-1/2, 1/2] (8e-8), n added to its exponent.  x below -126 counts as -126.
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
-  float a, b;
-  unpair(x2, a, b);
-  x2 = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  const uint64_t magic = pair(12582912.0f, 12582912.0f), t = add2(x2, magic);
-  const uint64_t n = add2(t, pair(-12582912.0f, -12582912.0f));
-  const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x2);
-  uint64_t y = fma2(f, pair(0.0013276472f, 0.0013276472f), pair(0.009675541f, 0.009675541f));
-  y = fma2(f, y, pair(0.05550713f, 0.05550713f));
-  y = fma2(f, y, pair(0.2402212f, 0.2402212f));
-  y = fma2(f, y, pair(0.69314694f, 0.69314694f));
-  y = fma2(f, y, pair(1.0000001f, 1.0000001f));
-  float u, v;
-  unpair(t, u, v);
-  unpair(y, a, b);
-  return pair(__uint_as_float(__float_as_uint(a) + (__float_as_uint(u) << 23)),
-              __uint_as_float(__float_as_uint(b) + (__float_as_uint(v) << 23)));
-}
-
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_long_kernel(const CrossParams p, const __grid_constant__ CUtensorMap k_map,
@@ -199,8 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar->v_clean, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->s_full[i], 1);
-      mbar_init(&bar->w_ready[i][0], 4);
-      mbar_init(&bar->w_ready[i][1], 4);
+      mbar_init(&bar->w_ready[i], 4);
       mbar_init(&bar->o_done[i], 1);
     }
     bar->stop = 0;
@@ -311,48 +290,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) mma_commit(b);
       __syncwarp();
     };
+    // A wait that gave up has set `stop`, which ends the others at once: the
+    // warp runs on, through MMAs on whatever is there, to the end.
+    auto wait = [&](uint64_t* b, int phase) { wait_for(bar, b, phase, p.status); };
     auto stage_ready = [&](int j) {
-      bool ok = wait_for(bar, &bar->full[j % kStages], (j / kStages) & 1, p.status);
-      if (ok && j + 1 == n && cut) ok = wait_for(bar, &bar->v_clean, 0, p.status);
-      return (bool)__all_sync(kFull, ok);
+      wait(&bar->full[j % kStages], (j / kStages) & 1);
+      if (j + 1 == n && cut) wait(&bar->v_clean, 0);
     };
-    bool ok = __all_sync(kFull, wait_for(bar, &bar->q_ready, 0, p.status) && wait_for(bar, &bar->k0_full, 0, p.status));
-    if (ok) {
-      tc_fence_after();
-      for (int i = 0; i < tiles; ++i) scores(i, kStages - 1);
-      commit(&bar->k0_done);
-      ok = stage_ready(0);
-    }
-    for (int j = 0; ok && j < n; ++j) {
+    wait(&bar->q_ready, 0);
+    wait(&bar->k0_full, 0);
+    tc_fence_after();
+    for (int i = 0; i < tiles; ++i) scores(i, kStages - 1);
+    commit(&bar->k0_done);
+    stage_ready(0);
+    for (int j = 0; j < n; ++j) {
       const int st = j % kStages;
       const uint64_t v = v_desc + 2 * st * kPart;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (i >= tiles || !ok) break;
+        if (i >= tiles) break;
         const uint32_t d = tmem + kO0 + 128 * i, w = tmem + kS0 + 128 * i;
+        wait(&bar->w_ready[i], j & 1);
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {  // the first 64 keys while the others' weights are made
-          ok = __all_sync(kFull, ok && wait_for(bar, &bar->w_ready[i][half], j & 1, p.status));
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-              mma_ts(d, w + 8 * (4 * half + s), v + (4 * half + s) * 128, kIdescO, j > 0 || half > 0 || s > 0);
-          }
-          __syncwarp();
+          for (int s = 0; s < 8; ++s) mma_ts(d, w + 8 * s, v + s * 128, kIdescO, j > 0 || s > 0);
         }
-        if (!ok) break;
-        if (j + 1 < n)
+        __syncwarp();
+        if (j + 1 < n) {
           scores(i, st);
-        else
+          if (i == 0) stage_ready(j + 1);
+        } else {
           commit(&bar->o_done[i]);
-        if (i == 0 && j + 1 < n) ok = stage_ready(j + 1);
+        }
       }
-      if (ok) commit(&bar->empty[st]);
+      commit(&bar->empty[st]);
     }
     // the last arrival lands before the block, and its barriers, are gone
-    if (ok) wait_for(bar, &bar->empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, p.status);
+    wait(&bar->empty[(n - 1) % kStages], ((n - 1) / kStages) & 1);
   } else if (warp >= 4 && live) {
     // ---- one query row per thread ----
     const int i = (warp - 4) >> 2, quarter = warp & 3, row_in = quarter * 32 + lane, row = row0 + 128 * i + row_in;
@@ -374,10 +349,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + lanes + kS0 + 128 * i, o_addr = tmem + lanes + kO0 + 128 * i;
     const float factor = __fmul_rn(p.scale, kLog2e);
     float top = -INFINITY, sum = 0.0f;
-    bool ok = steps > 0 && i < row_tiles;
-    for (int j = 0; ok && j < steps; ++j) {
-      ok = warp_wait(bar, &bar->s_full[i], j & 1, p.status);
-      if (!ok) break;
+    const bool used = steps > 0 && i < row_tiles;
+    bool ok = true;  // no wait gave up; the steps run on if one did, and the row is not written
+    for (int j = 0; used && j < steps; ++j) {
+      ok = wait_for(bar, &bar->s_full[i], j & 1, p.status) && ok;
+      __syncwarp();
       tc_fence_after();
       uint32_t s[4][32];
 #pragma unroll
@@ -423,46 +399,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t w[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          uint64_t x = fma2(pair(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1])), factor2, base2);
+          const uint64_t x = fma2(pair(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1])), factor2, base2);
           float a, e;
-          if (k % kPolyEvery == kPolyEvery - 1) {
-            x = exp2_pair(x);
-            unpair(x, a, e);
-          } else {
-            unpair(x, a, e);
-            a = exp2_approx(a);
-            e = exp2_approx(e);
-            x = pair(a, e);
-          }
-          add[k & 1] = add2(add[k & 1], x);
+          unpair(x, a, e);
+          a = exp2_approx(a);
+          e = exp2_approx(e);
+          add[k & 1] = add2(add[k & 1], pair(a, e));
           w[k] = BF16 ? pack_bf16(a, e) : pack_f16(a, e);
         }
         tmem_st_x16(s_addr + 16 * c, w);
-        if (c & 1) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive(&bar->w_ready[i][c >> 1]);
-        }
       }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(&bar->w_ready[i]);
       float a0, a1;
       unpair(add2(add[0], add[1]), a0, a1);
       sum = __fadd_rn(sum, __fadd_rn(a0, a1));
     }
-    if (ok) ok = warp_wait(bar, &bar->o_done[i], 0, p.status);
-    const bool written = i < row_tiles && (ok || steps <= 0);
+    if (used) ok = wait_for(bar, &bar->o_done[i], 0, p.status) && ok;
+    const bool written = i < row_tiles && ok && there;
     // ---- the row, normalized ----
     const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
     const float lse2 = sum == 0.0f ? -INFINITY : __fadd_rn(__fmul_rn(top, factor), log2f(sum));
     const bool direct = parts <= 1;
     const long long slot = ((long long)nth * kLongRows + 128 * i + row_in) * p.split.splits + split;
-    if (ok) tc_fence_after();
-    if (__any_sync(kFull, written && there)) {
+    __syncwarp();
+    tc_fence_after();
+    {
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
         uint32_t o[16];
         __syncwarp();
-        if (ok) {
+        if (used) {
           tmem_ld_x16(o_addr + 16 * c, o);
           tmem_ld_wait();
         } else {
@@ -472,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float f[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) f[k] = __fmul_rn(__uint_as_float(o[k]), inv);
-        if (direct && written && there) {
+        if (direct && written) {
           uint32_t w[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) w[k] = BF16 ? pack_bf16(f[2 * k], f[2 * k + 1]) : pack_f16(f[2 * k], f[2 * k + 1]);
@@ -480,13 +449,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                 (long long)h * r.out_head_stride + 16 * c);
           dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
           dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        } else if (written && there) {
+        } else if (written) {
           float4* dst = reinterpret_cast<float4*>(p.split.out + slot * D + 16 * c);
 #pragma unroll
           for (int k = 0; k < 4; ++k) dst[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
         }
       }
-      if (written && there) {
+      if (written) {
         if (!direct)
           p.split.lse[slot] = lse2;
         else if (r.lse)
