@@ -87,11 +87,14 @@ __device__ __forceinline__ uint32_t tf32_high(float x) { return (__float_as_uint
 __device__ __forceinline__ uint32_t tf32_low(float x) {
   return __float_as_uint(__fsub_rn(x, __uint_as_float(tf32_high(x))));
 }
-__device__ __forceinline__ void mma_split(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0,
-                                          float b1) {
+// d += high x high, rest += the products with a low part.  The tensor cores'
+// own additions do not round to nearest, so a sum of many terms drifts: the
+// small products have a sum of their own, and neither runs past one tile.
+__device__ __forceinline__ void mma_split(float (&d)[4], float (&rest)[4], const uint32_t (&ah)[4],
+                                          const uint32_t (&al)[4], float b0, float b1) {
   const uint32_t h0 = tf32_high(b0), h1 = tf32_high(b1);
-  mma_tf32(d, al, h0, h1);
-  mma_tf32(d, ah, tf32_low(b0), tf32_low(b1));
+  mma_tf32(rest, al, h0, h1);
+  mma_tf32(rest, ah, tf32_low(b0), tf32_low(b1));
   mma_tf32(d, ah, h0, h1);
 }
 
@@ -215,6 +218,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
       // (f32), so that a thread's two columns are the rows t and t + 4 of the
       // values, which lie in different banks
       if constexpr (kF32) {
+        float rest[kNT][4] = {};
 #pragma unroll
         for (int c = 0; c < D / 8; ++c) {
           uint32_t ah[4], al[4];
@@ -227,9 +231,13 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
           for (int j = 0; j < kNT; ++j) {
             if (8 * j >= keys) break;
             const float2 kv = *reinterpret_cast<const float2*>(ks + (8 * j + (g >> 1) + 4 * (g & 1)) * kPitch + 8 * c + 2 * t);
-            mma_split(x[j], ah, al, kv.x, kv.y);
+            mma_split(x[j], rest[j], ah, al, kv.x, kv.y);
           }
         }
+#pragma unroll
+        for (int j = 0; j < kNT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[j][e] = __fadd_rn(x[j][e], rest[j][e]);
       } else {
 #pragma unroll
         for (int c = 0; c < D / 16; ++c)
@@ -299,20 +307,31 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
         }
       // ---- values ----
       if constexpr (kF32) {
+        // k = t: column 2 t (key t); k = t + 4: column 2 t + 1 (key t + 4)
+        uint32_t ah[kNT][4], al[kNT][4];
 #pragma unroll
-        for (int j = 0; j < kNT; ++j) {
-          if (8 * j >= keys) break;
-          uint32_t ah[4], al[4];
-          // k = t: column 2 t (key t); k = t + 4: column 2 t + 1 (key t + 4)
-          ah[0] = tf32_high(x[j][0]); ah[1] = tf32_high(x[j][2]); ah[2] = tf32_high(x[j][1]); ah[3] = tf32_high(x[j][3]);
-          al[0] = tf32_low(x[j][0]); al[1] = tf32_low(x[j][2]); al[2] = tf32_low(x[j][1]); al[3] = tf32_low(x[j][3]);
-          const T* v0 = vs + (8 * j + t) * kPitch + 2 * g;
-          const T* v1 = v0 + 4 * kPitch;
+        for (int j = 0; j < kNT; ++j)
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            const float2 a = *reinterpret_cast<const float2*>(v0 + 16 * c), e = *reinterpret_cast<const float2*>(v1 + 16 * c);
-            mma_split(acc[2 * c], ah, al, a.x, e.x);
-            mma_split(acc[2 * c + 1], ah, al, a.y, e.y);
+          for (int e = 0; e < 4; ++e) {
+            const float w = x[j][e == 0 ? 0 : e == 1 ? 2 : e == 2 ? 1 : 3];
+            ah[j][e] = tf32_high(w);
+            al[j][e] = tf32_low(w);
+          }
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          float sum0[4] = {}, sum1[4] = {}, rest0[4] = {}, rest1[4] = {};
+#pragma unroll
+          for (int j = 0; j < kNT; ++j) {
+            if (8 * j >= keys) break;
+            const T* v0 = vs + (8 * j + t) * kPitch + 16 * c + 2 * g;
+            const float2 a = *reinterpret_cast<const float2*>(v0), e = *reinterpret_cast<const float2*>(v0 + 4 * kPitch);
+            mma_split(sum0, rest0, ah[j], al[j], a.x, e.x);
+            mma_split(sum1, rest1, ah[j], al[j], a.y, e.y);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[2 * c][e] = __fadd_rn(acc[2 * c][e], __fadd_rn(sum0[e], rest0[e]));
+            acc[2 * c + 1][e] = __fadd_rn(acc[2 * c + 1][e], __fadd_rn(sum1[e], rest1[e]));
           }
         }
       } else {
