@@ -323,7 +323,8 @@ mc_status mc_op_status(uint32_t *status_bits);
  * marian-cpu/src/q8_engine.rs:511-574) and picks the argmax (:749-790).
  *
  * Every pointer in the structs below is a device pointer of the current
- * device unless it says otherwise, arrays are dense unless they come with
+ * device (managed memory, or mapped host memory at its own address, will do;
+ * anything else is refused), arrays are dense unless they come with
  * strides, and strides count elements.  The struct itself is read during the
  * call.  The calls are asynchronous on `stream` (a cudaStream_t of the current
  * device, 0 = default), allocate nothing and can be captured in a CUDA graph

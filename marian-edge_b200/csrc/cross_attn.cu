@@ -603,8 +603,8 @@ extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* 
     return MC_INVALID_INPUT;
   const uint64_t need = mc_cross_attention_workspace(a);
   if (need > 0 && (!a->workspace || !mc::aligned16(a->workspace) || a->workspace_bytes < need)) return MC_INVALID_INPUT;
-  mc_status where = mc::on_current_device(a->q);
-  if (where == MC_OK) where = mc::on_current_device(a->k);
+  const mc_status where = mc::on_current_device({a->q, a->k, a->v, a->out, a->lse, a->q_start, a->q_len, a->k_start, a->k_len,
+                                                 a->key_mask, need > 0 ? a->workspace : nullptr});
   if (where != MC_OK) return where;
   uint32_t* status = mc::op_status_word();
   if (!status) return MC_CUDA;
@@ -644,5 +644,5 @@ extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* 
   cudaError_t e = cudaErrorNotSupported;
   if (mc::long_pays(a)) e = mc::launch_cross(p, mc::cross_plan(a, true), a->workspace, s);
   if (e == cudaErrorNotSupported) e = mc::launch_cross(p, mc::cross_plan(a, false), a->workspace, s);
-  return e == cudaSuccess ? MC_OK : MC_CUDA;
+  return mc::launched(e);
 }

@@ -8,6 +8,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 #include "marian_cuda.h"
 
@@ -142,19 +144,32 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 inline int dtype_bytes(int32_t dtype) { return dtype == MC_F32 ? 4 : dtype == MC_F16 || dtype == MC_BF16 ? 2 : 0; }
 
-// Memory of another device or pageable host memory is refused; memory that
-// CUDA says nothing about cannot be read by a kernel either.
-inline mc_status on_current_device(const void* p) {
+// Memory of another device or pageable host memory is refused, for every
+// pointer that is given (70 ns each); memory that CUDA says nothing about
+// cannot be read by a kernel either.
+inline mc_status on_current_device(std::initializer_list<const void*> pointers) {
   int dev = -1;
-  cudaPointerAttributes a;
   if (cudaGetDevice(&dev) != cudaSuccess) return MC_CUDA;
-  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
-    cudaGetLastError();
-    return MC_INVALID_INPUT;
+  for (const void* p : pointers) {
+    if (!p) continue;
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+      cudaGetLastError();
+      return MC_INVALID_INPUT;
+    }
+    const bool ours = a.type == cudaMemoryTypeDevice ? a.device == dev
+                                                     : a.type == cudaMemoryTypeManaged ||
+                                                           (a.type == cudaMemoryTypeHost && a.devicePointer == p);
+    if (!ours) return MC_INVALID_INPUT;
   }
-  if (a.type == cudaMemoryTypeDevice) return a.device == dev ? MC_OK : MC_INVALID_INPUT;
-  return a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeHost && a.devicePointer) ? MC_OK
-                                                                                             : MC_INVALID_INPUT;
+  return MC_OK;
+}
+
+// A launch's outcome; its error does not stay behind for the caller's own calls.
+inline mc_status launched(cudaError_t e) {
+  if (e == cudaSuccess) return MC_OK;
+  cudaGetLastError();
+  return MC_CUDA;
 }
 
 // Rows of head_dim values whose strides keep every 16-byte load aligned.

@@ -999,8 +999,7 @@ mc_status kv4_rows(const mc_kv4_cache* c, const mc_kv4_rows* a, void* stream) {
   if (READ && (!strides_apart(a->rows, c->kv_heads, c->head_dim, a->k_row_stride, a->k_head_stride) ||
                !strides_apart(a->rows, c->kv_heads, c->head_dim, a->v_row_stride, a->v_head_stride) || a->k == a->v))
     return MC_INVALID_INPUT;
-  mc_status where = on_current_device(c->pages);
-  if (where == MC_OK) where = on_current_device(a->k);
+  const mc_status where = on_current_device({c->pages, c->page_table, a->k, a->v, a->start, a->count, a->first});
   if (where != MC_OK) return where;
   uint32_t* status = op_status_word();
   if (!status) return MC_CUDA;
@@ -1011,7 +1010,7 @@ mc_status kv4_rows(const mc_kv4_cache* c, const mc_kv4_rows* a, void* stream) {
   const cudaError_t e = a->dtype == MC_F32   ? launch_rows_l<MC_F32, READ>(pool, r, grid, (int)chunks, status, s)
                         : a->dtype == MC_F16 ? launch_rows_l<MC_F16, READ>(pool, r, grid, (int)chunks, status, s)
                                              : launch_rows_l<MC_BF16, READ>(pool, r, grid, (int)chunks, status, s);
-  return e == cudaSuccess ? MC_OK : MC_CUDA;
+  return launched(e);
 }
 
 }  // namespace
@@ -1058,8 +1057,8 @@ extern "C" mc_status mc_kv4_attention(const mc_kv4_cache* c, const mc_kv4_attent
     return MC_INVALID_INPUT;
   if (plan.bytes > 0 && (!a->workspace || !mc::aligned16(a->workspace) || a->workspace_bytes < plan.bytes))
     return MC_INVALID_INPUT;
-  mc_status where = mc::on_current_device(c->pages);
-  if (where == MC_OK) where = mc::on_current_device(a->q);
+  const mc_status where = mc::on_current_device({c->pages, c->page_table, a->q, a->out, a->lse, a->q_start, a->q_len,
+                                                 a->kv_len, plan.bytes > 0 ? a->workspace : nullptr});
   if (where != MC_OK) return where;
   uint32_t* status = mc::op_status_word();
   if (!status) return MC_CUDA;
@@ -1109,8 +1108,7 @@ extern "C" mc_status mc_kv4_attention(const mc_kv4_cache* c, const mc_kv4_attent
     case 112: e = mc::launch_kv4_attn_d<112>(p, plan, s); break;
     case 128: e = mc::launch_kv4_attn_d<128>(p, plan, s); break;
   }
-  if (e != cudaSuccess) return MC_CUDA;
-  if (plan.splits > 1)
+  if (e == cudaSuccess && plan.splits > 1)
     e = mc::launch_attn_join(r, p.split, mc::kTileKeys, plan.nt * (a->dtype == MC_F32 ? 4 : 8), plan.row_tiles, s);
-  return e == cudaSuccess ? MC_OK : MC_CUDA;
+  return mc::launched(e);
 }

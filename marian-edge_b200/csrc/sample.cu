@@ -1085,8 +1085,8 @@ extern "C" mc_status mc_sample(const mc_sample_args* a, void* stream) {
       !mc::aligned4(a->tokens) || !mc::aligned4(a->probs) || !mc::aligned4(a->candidates) ||
       (a->candidates && (a->candidates_stride < 0 || a->candidates_stride >= (int64_t(1) << 40))))
     return MC_INVALID_INPUT;
-  mc_status where = mc::on_current_device(a->logits);
-  if (where == MC_OK) where = mc::on_current_device(a->tokens);
+  const mc_status where = mc::on_current_device({a->logits, a->temperature, a->top_k, a->top_p, a->min_p, a->uniform,
+                                                 a->candidates, a->tokens, a->probs});
   if (where != MC_OK) return where;
   mc::SampleParams p;
   std::memset(&p, 0, sizeof(p));
@@ -1109,5 +1109,5 @@ extern "C" mc_status mc_sample(const mc_sample_args* a, void* stream) {
   const cudaError_t e = a->dtype == MC_F32   ? mc::launch_sample<float>(p, s)
                         : a->dtype == MC_F16 ? mc::launch_sample<__half>(p, s)
                                              : mc::launch_sample<__nv_bfloat16>(p, s);
-  return e == cudaSuccess ? MC_OK : MC_CUDA;
+  return mc::launched(e);
 }

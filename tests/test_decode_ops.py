@@ -114,3 +114,48 @@ def test_sampled_translations_step_by_step(src_len, copies):
     assert status_bits() == 0
     if copies > 1:   # the copies of a source draw different translations
         assert len({int(x) for x in tokens}) > 1
+
+
+def test_host_memory_is_refused_wherever_it_is_given():
+    # every pointer but the one in question is good; nothing is launched
+    lib = L.load()
+    host = torch.zeros(4096, dtype=torch.uint8)
+    at = (host.data_ptr() + 15) // 16 * 16
+    room = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    base = room.data_ptr()
+    zeros = room[:64].data_ptr()
+
+    def refused(call, struct, fields):
+        for f in fields:
+            keep = getattr(struct, f)
+            setattr(struct, f, at)
+            assert call() == L.MC_INVALID_INPUT, f
+            setattr(struct, f, keep)
+        assert call() == L.MC_OK
+
+    cache = L.Kv4Cache(pages=base, page_table=zeros, n_pages=4, page_tokens=16, kv_heads=1, head_dim=64, batch=1,
+                       pages_per_seq=2)
+    rows = L.Kv4Rows(k=base + 65536, v=base + 131072, start=zeros, count=zeros, first=zeros, rows=8, k_row_stride=64,
+                     k_head_stride=64, v_row_stride=64, v_head_stride=64, dtype=L.MC_F32, max_count=4)
+    for fn in (lib.mc_kv4_append, lib.mc_kv4_read):
+        refused(lambda: fn(C.byref(cache), C.byref(rows), None), rows, ["k", "v", "start", "count", "first"])
+        refused(lambda: fn(C.byref(cache), C.byref(rows), None), cache, ["pages", "page_table"])
+    att = L.Kv4AttentionArgs(q=base + 65536, out=base + 131072, lse=base + 4096, q_start=zeros, q_len=zeros,
+                             kv_len=zeros, q_rows=8, q_row_stride=64, q_head_stride=64, out_row_stride=64,
+                             out_head_stride=64, dtype=L.MC_F32, heads=1, max_q_len=1, max_kv_len=32, scale=1.0)
+    refused(lambda: lib.mc_kv4_attention(C.byref(cache), C.byref(att), None), att,
+            ["q", "out", "lse", "q_start", "q_len", "kv_len"])
+    cross = L.CrossAttentionArgs(q=base + 65536, k=base + 131072, v=base + 196608, out=base + 262144, lse=base + 4096,
+                                 q_start=zeros, q_len=zeros, k_start=zeros, k_len=zeros, key_mask=zeros, q_rows=8,
+                                 k_rows=8, q_row_stride=64, q_head_stride=64, k_row_stride=64, k_head_stride=64,
+                                 v_row_stride=64, v_head_stride=64, out_row_stride=64, out_head_stride=64,
+                                 dtype=L.MC_F32, batch=1, heads=1, kv_heads=1, head_dim=64, max_q_len=1, max_k_len=8,
+                                 scale=1.0)
+    refused(lambda: lib.mc_cross_attention(C.byref(cross), None), cross,
+            ["q", "k", "v", "out", "lse", "q_start", "q_len", "k_start", "k_len", "key_mask"])
+    draw = L.SampleArgs(logits=base + 65536, temperature=zeros, top_k=zeros, top_p=zeros, min_p=zeros, uniform=zeros,
+                        tokens=base + 8192, probs=base + 12288, row_stride=100, dtype=L.MC_F32, rows=1, vocab=100)
+    refused(lambda: lib.mc_sample(C.byref(draw), None), draw,
+            ["logits", "temperature", "top_k", "top_p", "min_p", "uniform", "candidates", "tokens", "probs"])
+    torch.cuda.synchronize()
+    assert status_bits() == 0
