@@ -145,18 +145,22 @@ __device__ __forceinline__ void row_range(const Eight<TYPE>& x, bool live, float
 // quotient.  A single-precision quotient is within 3e-6 of it for codes up to
 // 16, so only one that lands within 1e-5 of a half needs the double-precision
 // one, whose ties are exact (the scale has 11 significant bits).  Rounding is
-// the addition of 1.5 * 2^23; four codes are one exact float.
+// the addition of 1.5 * 2^23; six codes are one exact float.
 __device__ __forceinline__ uint32_t codes_of(const float (&f)[8], float minimum, float scale) {
   const float inverse = __frcp_rn(scale);
-  float c[8];
-  bool near_half = false;
+  const uint64_t minus = pair(-minimum, -minimum), times = pair(inverse, inverse), magic = pair(12582912.0f, 12582912.0f);
+  uint64_t c[4];
+  float off = 0.0f;  // how far the quotients are from whole numbers, at most
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(f[i], minimum), inverse), 0.0f), 15.0f);
-    c[i] = __fsub_rn(__fadd_rn(t, 12582912.0f), 12582912.0f);
-    near_half |= fabsf(__fsub_rn(t, c[i])) > 0.49999f;
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    unpair(mul2(add2(pair(f[2 * i], f[2 * i + 1]), minus), times), a, b);
+    const uint64_t t = pair(fminf(fmaxf(a, 0.0f), 15.0f), fminf(fmaxf(b, 0.0f), 15.0f));
+    c[i] = add2(add2(t, magic), pair(-12582912.0f, -12582912.0f));
+    unpair(fma2(c[i], pair(-1.0f, -1.0f), t), a, b);
+    off = fmaxf(off, fmaxf(fabsf(a), fabsf(b)));
   }
-  if (near_half) {
+  if (off > 0.49999f) {
 #pragma unroll 1
     for (int i = 0; i < 8; ++i) {
       float x = f[0];
@@ -164,22 +168,22 @@ __device__ __forceinline__ uint32_t codes_of(const float (&f)[8], float minimum,
       for (int j = 1; j < 8; ++j) x = i == j ? f[j] : x;
       const float r = (float)fmin(fmax(rint(__ddiv_rn(__dsub_rn((double)x, (double)minimum), (double)scale)), 0.0), 15.0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) c[j] = i == j ? r : c[j];
+      for (int j = 0; j < 4; ++j) {
+        float a, b;
+        unpair(c[j], a, b);
+        c[j] = pair(i == 2 * j ? r : a, i == 2 * j + 1 ? r : b);
+      }
     }
   }
-  uint32_t half[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float v = __fmaf_rn(c[4 * k + 3], 16.0f, c[4 * k + 2]);
-    v = __fmaf_rn(v, 16.0f, c[4 * k + 1]);
-    v = __fmaf_rn(v, 16.0f, c[4 * k]);
-    half[k] = __float_as_uint(__fadd_rn(v, 8388608.0f));
-  }
-  return __byte_perm(half[0], half[1], 0x5410);
+  const uint64_t p256 = pair(256.0f, 256.0f);
+  float even, odd, c6, c7;
+  unpair(fma2(fma2(c[2], p256, c[1]), p256, c[0]), even, odd);
+  unpair(c[3], c6, c7);
+  return (uint32_t)__fmaf_rn(odd, 16.0f, even) | (uint32_t)__fmaf_rn(c7, 16.0f, c6) << 24;
 }
 
 template <int TYPE, int L, bool READ>
-__global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const Kv4Pool p, const Kv4RowsDev r, int chunks,
+__global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const Kv4Pool p, const Kv4RowsDev r, int chunks,
                                                                uint32_t* status) {
   pdl_enter();
   const int b = blockIdx.x / chunks, chunk = blockIdx.x - b * chunks;
@@ -203,57 +207,64 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const Kv4Pool p, 
     const bool mine = h < p.kv_heads && active;
     const long long rs = (which ? r.v_rs : r.k_rs) * kBytes;
     char* x0 = static_cast<char*>(which ? r.v : r.k) + (start + t0) * rs + (h * (which ? r.v_hs : r.k_hs) + lane * 8) * kBytes;
-    for (int t = 0; t < nt; t += kRowsInFlight) {
-      Eight<TYPE> x[kRowsInFlight];
-      uint32_t word[kRowsInFlight];
-      __half2 pair[kRowsInFlight];
-      uint8_t* block[kRowsInFlight];  // of the row's page and head; nullptr: no row
-#pragma unroll
-      for (int u = 0; u < kRowsInFlight; ++u) {
-        block[u] = nullptr;
-        const int pos = first + t0 + t + u;
-        if (!mine || t + u >= nt) continue;
-        const long long page = table[pos >> p.token_shift];
-        if (page < 0 || page >= p.n_pages) {
-          bad_page = true;
-          continue;
-        }
-        block[u] = p.pages + (page * p.kv_heads + h) * block_bytes;
-        const int slot = which * tokens + (pos & (tokens - 1));
-        if (READ) {
-          word[u] = __ldcs(reinterpret_cast<const uint32_t*>(block[u] + slot * (d / 2)) + lane);
-          pair[u] = reinterpret_cast<const __half2*>(block[u] + tokens * d)[slot];
-        } else {
-          x[u].load(x0 + (t + u) * rs);
-        }
+    // The rows that lie in one page follow one another in it.
+    for (int t = 0, run; t < nt; t += run) {
+      const int pos = first + t0 + t, in_page = pos & (tokens - 1);
+      run = min(tokens - in_page, nt - t);
+      const long long page = table[pos >> p.token_shift];
+      if (page < 0 || page >= p.n_pages) {
+        bad_page = true;
+        continue;
       }
+      uint8_t* block = p.pages + (page * p.kv_heads + h) * block_bytes;
+      uint8_t* codes = block + (which * tokens + in_page) * (d / 2) + lane * 4;
+      __half2* pairs = reinterpret_cast<__half2*>(block + tokens * d) + which * tokens + in_page;
+      char* from = x0 + t * rs;
+      for (int done = 0; done < run; done += kRowsInFlight) {
+        Eight<TYPE> x[kRowsInFlight];
+        uint32_t word[kRowsInFlight];
+        __half2 pair[kRowsInFlight];
 #pragma unroll
-      for (int u = 0; u < kRowsInFlight; ++u) {
-        const int slot = which * tokens + ((first + t0 + t + u) & (tokens - 1));
-        float f[8];
-        if (READ) {
-          if (!block[u]) continue;
-          const float scale = __low2float(pair[u]), minimum = __high2float(pair[u]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = __fmaf_rn(scale, (float)((word[u] >> (4 * i)) & 15), minimum);
-          store_eight<TYPE>(x0 + (t + u) * rs, f);
-        } else {
-          float low, high;
-          row_range<TYPE, L>(x[u], block[u] != nullptr, &low, &high);
-          if (!block[u]) continue;
-          __half min_h = __float2half_rn(low);
-          __half scale_h = __float2half_rn(__fmul_rn(__fsub_rn(high, __half2float(min_h)), 1.0f / 15.0f));
-          uint32_t w = 0;
-          if (__hisinf(min_h) || __hisinf(scale_h) || __hisnan(scale_h)) {
-            bad = true;
-            min_h = scale_h = __float2half_rn(0.0f);
-          } else if (__half2float(scale_h) > 0.0f) {
-            x[u].values(f);
-            w = codes_of(f, __half2float(min_h), __half2float(scale_h));
+        for (int u = 0; u < kRowsInFlight; ++u) {
+          if (!mine || done + u >= run) continue;
+          if (READ) {
+            word[u] = __ldcs(reinterpret_cast<const uint32_t*>(codes + u * (d / 2)));
+            pair[u] = pairs[u];
+          } else {
+            x[u].load(from + u * rs);
           }
-          reinterpret_cast<uint32_t*>(block[u] + slot * (d / 2))[lane] = w;
-          if (lane == 0) reinterpret_cast<__half2*>(block[u] + tokens * d)[slot] = __halves2half2(scale_h, min_h);
         }
+#pragma unroll
+        for (int u = 0; u < kRowsInFlight; ++u) {
+          const bool live = mine && done + u < run;
+          float f[8];
+          if (READ) {
+            if (!live) continue;
+            const float scale = __low2float(pair[u]), minimum = __high2float(pair[u]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __fmaf_rn(scale, (float)((word[u] >> (4 * i)) & 15), minimum);
+            store_eight<TYPE>(from + u * rs, f);
+          } else {
+            float low, high;
+            row_range<TYPE, L>(x[u], live, &low, &high);
+            if (!live) continue;
+            __half min_h = __float2half_rn(low);
+            __half scale_h = __float2half_rn(__fmul_rn(__fsub_rn(high, __half2float(min_h)), 1.0f / 15.0f));
+            uint32_t w = 0;
+            if (__hisinf(min_h) || __hisinf(scale_h) || __hisnan(scale_h)) {
+              bad = true;
+              min_h = scale_h = __float2half_rn(0.0f);
+            } else if (__half2float(scale_h) > 0.0f) {
+              x[u].values(f);
+              w = codes_of(f, __half2float(min_h), __half2float(scale_h));
+            }
+            *reinterpret_cast<uint32_t*>(codes + u * (d / 2)) = w;
+            if (lane == 0) pairs[u] = __halves2half2(scale_h, min_h);
+          }
+        }
+        codes += kRowsInFlight * (d / 2);
+        pairs += kRowsInFlight;
+        from += kRowsInFlight * rs;
       }
     }
   }
