@@ -101,6 +101,7 @@ __device__ __forceinline__ void mma_split(float (&d)[4], float (&rest)[4], const
 template <typename T, int D, int WR>
 __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
   constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int kType = kF32 ? MC_F32 : std::is_same<T, __half>::value ? MC_F16 : MC_BF16;
   constexpr int kKeys = Tile<T>::kKeys, kGroups = 4 / WR, kOwn = kKeys / kGroups, kNT = kOwn / 8;
   constexpr int kPitch = pitch<T, D>(), kElems = stage_elems<T, D>(), kRows = 16 * WR;
   constexpr int kChunk = 16 / (int)sizeof(T), kRowChunks = D / kChunk;
@@ -113,14 +114,14 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
   pdl_enter();
 
   const AttnRows& r = p.rows;
-  const uint32_t unit = blockIdx.x, bh = unit / (uint32_t)p.row_tiles;
-  const int tile = (int)(unit - bh * p.row_tiles), b = (int)(bh / (uint32_t)r.kv_heads), head = (int)(bh - (uint32_t)b * r.kv_heads);
+  const uint32_t unit = blockIdx.x, bh = share(unit, (uint32_t)p.row_tiles);
+  const int tile = (int)(unit - bh * p.row_tiles), b = (int)share(bh, (uint32_t)r.kv_heads), head = (int)(bh - (uint32_t)b * r.kv_heads);
   const int split = blockIdx.y;
   const AttnSeq seq = attn_seq(r, b, p.status, head == 0 && tile == 0 && split == 0 && tid == 0);
   const int n_rows = seq.nq * r.group, row0 = tile * kRows;
   if (!seq.ok || row0 >= n_rows) return;
   const int n_tiles = (seq.nk + kKeys - 1) / kKeys;
-  const int parts = max(1, (n_tiles + p.split.chunk - 1) / p.split.chunk);
+  const int parts = p.split.splits == 1 ? 1 : max(1, (n_tiles + p.split.chunk - 1) / p.split.chunk);
   if (split >= parts) return;
   const int begin = split * p.split.chunk, end = min(n_tiles, begin + p.split.chunk);
 
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
   for (int h = 0; h < 2; ++h) {
     const int row = own + g + 8 * h;
     there[h] = row < n_rows;
-    const int pos = there[h] ? (int)((uint32_t)row / (uint32_t)r.group) : 0, qh = head * r.group + (there[h] ? row - pos * r.group : 0);
+    const int pos = there[h] ? (int)share((uint32_t)row, (uint32_t)r.group) : 0, qh = head * r.group + (there[h] ? row - pos * r.group : 0);
     src[h] = static_cast<const T*>(r.q) + (long long)(seq.q0 + pos) * r.q_row_stride + (long long)qh * r.q_head_stride;
   }
   const bool busy = own < n_rows;
@@ -378,13 +379,13 @@ __global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
   };
   auto place_of = [&](int row) {  // of the unit
     if (!direct) return Place{((slot0 + row) * p.split.splits + split) * D, (slot0 + row) * p.split.splits + split};
-    const int pos = (int)((uint32_t)(row0 + row) / (uint32_t)r.group), h = head * r.group + (row0 + row) - pos * r.group;
+    const int pos = (int)share((uint32_t)(row0 + row), (uint32_t)r.group), h = head * r.group + (row0 + row) - pos * r.group;
     return Place{(long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride,
                  (long long)(seq.q0 + pos) * r.kv_heads * r.group + h};
   };
   auto emit = [&](const Place& to, int ch, float a, float e) {
     if (direct)
-      store2(r.out, to.out + ch, r.dtype, a, e);
+      store2(r.out, to.out + ch, kType, a, e);
     else
       *reinterpret_cast<float2*>(p.split.out + to.out + ch) = make_float2(a, e);
   };

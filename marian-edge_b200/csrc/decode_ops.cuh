@@ -116,6 +116,10 @@ struct AttnRows {
   int dtype, batch, kv_heads, group, head_dim, max_q, max_k, causal;
 };
 
+// a / d for the divisors that are mostly 1 (heads of a group, row tiles): a
+// division is some twenty instructions, and a short unit has several.
+__device__ __forceinline__ uint32_t share(uint32_t a, uint32_t d) { return d == 1 ? a : a / d; }
+
 struct AttnSeq {
   int q0, nq, k0, nk;
   bool ok;

@@ -375,15 +375,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
   pdl_enter();
 
   const AttnRows& r = p.rows;
+  const int dtype = SPLIT ? (int)MC_F32 : r.dtype;
   const int wpu = 1 << p.warps_log2, sub = warp & (wpu - 1);
   const uint32_t unit = blockIdx.x * (kAttnWarps >> p.warps_log2) + (warp >> p.warps_log2);
   const int split = blockIdx.y;
   bool live = unit < p.units;
   int b = 0, head = 0, tile = 0;
   if (live) {
-    const uint32_t bh = unit / (uint32_t)p.row_tiles;
+    const uint32_t bh = share(unit, (uint32_t)p.row_tiles);
     tile = (int)(unit - bh * p.row_tiles);
-    b = (int)(bh / (uint32_t)r.kv_heads);
+    b = (int)share(bh, (uint32_t)r.kv_heads);
     head = (int)(bh - (uint32_t)b * r.kv_heads);
   }
   AttnSeq seq = {0, 0, 0, 0, false};
@@ -391,11 +392,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
   const int n_rows = seq.nq * r.group, row0 = tile * kQ;
   live = live && row0 < n_rows;
   // The keys that the unit's last query sees, and this warp's tiles of them.
-  const int pos_last = live ? min(seq.nq - 1, (int)((uint32_t)(row0 + kQ - 1) / (uint32_t)r.group)) : 0;
-  const int pos_first = live ? (int)((uint32_t)row0 / (uint32_t)r.group) : 0;
+  const int pos_last = live ? min(seq.nq - 1, (int)share((uint32_t)(row0 + kQ - 1), (uint32_t)r.group)) : 0;
+  const int pos_first = live ? (int)share((uint32_t)row0, (uint32_t)r.group) : 0;
   const int keys = live ? max(0, r.causal ? seq.nk - (seq.nq - 1 - pos_last) : seq.nk) : 0;
   const int keys_all = live ? max(0, r.causal ? seq.nk - (seq.nq - 1 - pos_first) : seq.nk) : 0;  // seen by every query
-  const int splits_here = live ? max(1, ((seq.nk + kTileKeys - 1) / kTileKeys + p.split.chunk - 1) / p.split.chunk) : 0;
+  const int splits_here = !live                 ? 0
+                          : p.split.splits == 1 ? 1
+                                                : max(1, ((seq.nk + kTileKeys - 1) / kTileKeys + p.split.chunk - 1) / p.split.chunk);
   live = live && split < splits_here;
   const int n_tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int lo = min(n_tiles, split * p.split.chunk), hi = min(n_tiles, lo + p.split.chunk);
@@ -411,17 +414,17 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
   for (int n = 0; n < NT; ++n) {
     const int row = row0 + n * kCols + col;
     const bool there = live && row < n_rows;
-    const int pos = there ? (int)((uint32_t)row / (uint32_t)r.group) : 0, h = head * r.group + (there ? row - pos * r.group : 0);
+    const int pos = there ? (int)share((uint32_t)row, (uint32_t)r.group) : 0, h = head * r.group + (there ? row - pos * r.group : 0);
     const char* src = static_cast<const char*>(r.q) +
                       ((long long)(seq.q0 + pos) * r.q_row_stride + (long long)h * r.q_head_stride) *
-                          (r.dtype == MC_F32 ? 4 : 2);
+                          (SPLIT ? 4 : 2);
     // words t * (D / 32) + c of the whole 32-channel blocks, then the tail's four channels
     float f[kSteps * 4];
     constexpr int kWhole = (D / 32) * 8;
 #pragma unroll
     for (int i = 0; i < kSteps * 4; i += 2) {
       const int ch = i < kWhole ? t * kWhole + i : (D / 32) * 32 + 4 * t + i - kWhole;
-      const float2 v = there ? load2(src, ch, r.dtype) : make_float2(0.0f, 0.0f);
+      const float2 v = there ? load2(src, ch, dtype) : make_float2(0.0f, 0.0f);
       f[i] = v.x;
       f[i + 1] = v.y;
     }
@@ -765,7 +768,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = min(row0 + n * kCols + 2 * t + j, max(n_rows - 1, 0));
-      const int pos = (int)((uint32_t)row / (uint32_t)r.group), h = head * r.group + row - pos * r.group;
+      const int pos = (int)share((uint32_t)row, (uint32_t)r.group), h = head * r.group + row - pos * r.group;
       at[j] = direct ? (long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride
                      : ((slot0 + n * kCols + 2 * t + j) * p.split.splits + split) * D;
     }
@@ -796,7 +799,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
         if (join) {
           *reinterpret_cast<float2*>(own_out + q * D + 2 * byte) = make_float2(even, odd);
         } else if (direct) {
-          store2(r.out, at[j] + 2 * byte, r.dtype, even, odd);
+          store2(r.out, at[j] + 2 * byte, dtype, even, odd);
         } else {
           *reinterpret_cast<float2*>(p.split.out + at[j] + 2 * byte) = make_float2(even, odd);
         }
@@ -810,7 +813,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
         if (join) {
           own_lse[q] = lse2[j];
         } else if (direct) {
-          const int pos = (row0 + q) / r.group, h = head * r.group + (row0 + q) - pos * r.group;
+          const int pos = (int)share((uint32_t)(row0 + q), (uint32_t)r.group), h = head * r.group + (row0 + q) - pos * r.group;
           if (r.lse) r.lse[(long long)(seq.q0 + pos) * r.kv_heads * r.group + h] = __fmul_rn(lse2[j], kLn2);
         } else {
           p.split.lse[(slot0 + q) * p.split.splits + split] = lse2[j];
@@ -836,7 +839,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
       total = __fadd_rn(total, l[w]);
     }
     const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
-    const int pos = (row0 + q) / r.group, h = head * r.group + (row0 + q) - pos * r.group;
+    const int pos = (int)share((uint32_t)(row0 + q), (uint32_t)r.group), h = head * r.group + (row0 + q) - pos * r.group;
     for (int c = 2 * lane; c < D; c += 64) {
       float a = 0.0f, e = 0.0f;
 #pragma unroll
@@ -850,7 +853,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
       a = __fmul_rn(a, inv);
       e = __fmul_rn(e, inv);
       if (direct)
-        store2(r.out, (long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride + c, r.dtype, a,
+        store2(r.out, (long long)(seq.q0 + pos) * r.out_row_stride + (long long)h * r.out_head_stride + c, dtype, a,
                e);
       else
         *reinterpret_cast<float2*>(p.split.out + ((slot0 + q) * p.split.splits + split) * D + c) = make_float2(a, e);
