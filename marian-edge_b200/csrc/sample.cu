@@ -644,9 +644,11 @@ __device__ void finish_list(Row<T>& r, const Weigher& weigh, const Cuts& q, int 
   for (int j = 0; j < kEach; ++j) {
     weight[j] = 0;
     if (first + j < in_a) {
-      const double real = weigh.near(value_of((uint32_t)(sh.list[first + j] >> 32)));
+      const uint32_t key = (uint32_t)(sh.list[first + j] >> 32);
+      const double real = weigh.near(value_of(key));
       weight[j] = Weigher::fixed(real);
-      above_floor += real >= q.floor_w;
+      // the largest logit's weight is 1, from which near() may be a rounding off
+      above_floor += key == weigh.top_key || real >= q.floor_w;
     }
     sum += weight[j];
   }

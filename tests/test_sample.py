@@ -328,3 +328,17 @@ def test_captured_and_replayed_on_new_logits():
         torch.cuda.synchronize()
         want, _ = sample(x, u=u.cpu().numpy())
         assert (tokens.cpu().numpy() == want).all()
+
+
+@gpu
+@pytest.mark.parametrize("top_k", [0, 50])
+def test_min_p_of_one_keeps_the_largest(top_k):
+    # whatever (largest - largest) / temperature comes out as in double: with
+    # largest / temperature rounded, half of the rows lie below 1
+    rng = np.random.default_rng(15)
+    rows, vocab = 64, 3000
+    x = rng.standard_normal((rows, vocab)) * 5 + 10
+    x[::3, 40] = x[::3, 2900] = 60.0       # the largest, twice
+    x[::5, 1000:1400] = 70.0               # and 400 times
+    check(x, rng.uniform(0.3, 2.0, rows), np.full(rows, top_k), None, np.ones(rows), rng.random(rows))
+    assert status_bits() == 0
