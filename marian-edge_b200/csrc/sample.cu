@@ -1007,7 +1007,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   }
 
   // ---- the general way: top-k, then top-p ----
-  const uint32_t key_min = max(kKeyNone + 1, key_of(__fsub_rn(top, reach)));
+  // (an infinite logit less an infinite reach is no number: only its ties count)
+  const uint32_t key_min = top == INFINITY ? key_max : max(kKeyNone + 1, key_of(__fsub_rn(top, reach)));
   auto fixed_weight = [&](float v, uint32_t k) -> unsigned long long {
     if (!regular) return Weigher::fixed(weigh.real(v, k));
     const unsigned long long w = Weigher::fixed(weigh.near(v));

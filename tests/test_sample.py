@@ -342,3 +342,15 @@ def test_min_p_of_one_keeps_the_largest(top_k):
     x[::5, 1000:1400] = 70.0               # and 400 times
     check(x, rng.uniform(0.3, 2.0, rows), np.full(rows, top_k), None, np.ones(rows), rng.random(rows))
     assert status_bits() == 0
+
+
+@gpu
+def test_infinite_logits_at_an_infinite_temperature():
+    rows, vocab = 6, 900
+    x = np.repeat(np.random.default_rng(16).standard_normal((1, vocab)), rows, 0)
+    x[:, [11, 500, 800]] = np.inf
+    t = np.array([np.inf, np.inf, np.inf, 3e37, 3e37, 1.0])
+    k, p = np.array([1, 2, 0, 1, 0, 2]), np.array([1.0, 1.0, 0.6, 1.0, 0.2, 1.0])
+    tokens, probs = sample(torch.from_numpy(x.astype(np.float32)).cuda(), t, k, p, None, np.full(rows, 0.75))
+    assert tokens.tolist() == [11, 500, 500, 11, 11, 500]
+    assert probs.tolist() == [1.0, 0.5, 0.5, 1.0, 1.0, 0.5]
