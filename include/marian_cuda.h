@@ -407,7 +407,7 @@ typedef struct {
     int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
     int32_t dtype;               /* mc_dtype of q and out */
     int32_t heads;               /* a multiple of the cache's kv_heads */
-    int32_t max_q_len, max_kv_len;  /* no q_len[b] / kv_len[b] is above them */
+    int32_t max_q_len, max_kv_len;  /* no q_len[b] / kv_len[b] is above them; max_kv_len <= 2^31 - 256 */
     int32_t causal;
     float scale;                 /* finite, commonly 1 / sqrt(head_dim) */
 } mc_kv4_attention_args;
@@ -444,7 +444,7 @@ typedef struct {
     int32_t dtype;               /* mc_dtype of q, k, v and out */
     int32_t batch, heads, kv_heads;  /* heads a multiple of kv_heads */
     int32_t head_dim;            /* a multiple of 16, 16..128 */
-    int32_t max_q_len, max_k_len;  /* no q_len[b] / k_len[b] is above them */
+    int32_t max_q_len, max_k_len;  /* no q_len[b] / k_len[b] is above them; max_k_len <= 2^31 - 256 */
     float scale;                 /* finite, commonly 1 / sqrt(head_dim) */
 } mc_cross_attention_args;
 

@@ -20,6 +20,7 @@ namespace mc {
 uint32_t* op_status_word();
 
 constexpr int kOpMaxHeadDim = 128;
+constexpr int kOpMaxKeys = INT32_MAX - 255;  // of a sequence: positions a tile further on still are an int
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -942,7 +942,7 @@ bool kv4_cache_ok(const mc_kv4_cache* c) {
 // two tiles (of 32 keys), as a join costs about as much as a tile.
 bool kv4_plan(const mc_kv4_cache* c, const mc_kv4_attention_args* a, Kv4Plan* plan) {
   if (!kv4_cache_ok(c) || !a || dtype_bytes(a->dtype) == 0 || a->heads < 1 || a->heads % c->kv_heads != 0 ||
-      a->max_q_len < 0 || a->max_kv_len < 0)
+      a->max_q_len < 0 || a->max_kv_len < 0 || a->max_kv_len > kOpMaxKeys)
     return false;
   const int64_t group = a->heads / c->kv_heads, rows = group * a->max_q_len;
   if (rows > INT32_MAX / 2) return false;

@@ -383,3 +383,14 @@ def test_long_sequences_in_several_waves(h, hk, cut):
     assert (need > 0) == cut
     need = check(rng, [512] * 9 + [300, 0, 256, 257], [1100] * 11 + [130, 0], h, hk, 32, "bf16")
     assert (need > 0) == cut
+
+
+def test_key_counts_next_to_the_largest_integer():
+    # a tile's last position has to be an int too
+    lib, a = L.load(), host_args()
+    a.k_rows = a.max_k_len = 2**31 - 256
+    assert lib.mc_cross_attention_workspace(C.byref(a)) > 0
+    for n in (2**31 - 255, 2**31 - 1):
+        a.k_rows = a.max_k_len = n
+        assert lib.mc_cross_attention_workspace(C.byref(a)) == 0
+        assert lib.mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT

@@ -671,3 +671,15 @@ def test_two_streams_and_a_captured_step():
         assert torch.equal(out0, out1) and torch.equal(out0, out2)
         assert torch.equal(caches[0].pages, caches[1].pages)
     assert status_bits() == 0
+
+
+def test_key_counts_next_to_the_largest_integer():
+    # a tile's last position has to be an int too
+    lib, (cache, _, att) = L.load(), host_args()
+    cache.page_tokens, cache.pages_per_seq = 8, 2**28 - 1
+    att.max_kv_len = 2**31 - 256
+    assert lib.mc_kv4_attention_workspace(C.byref(cache), C.byref(att)) > 0
+    for n in (2**31 - 255, 2**31 - 8):
+        att.max_kv_len = n
+        assert lib.mc_kv4_attention_workspace(C.byref(cache), C.byref(att)) == 0
+        assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == L.MC_INVALID_INPUT
