@@ -940,7 +940,9 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   }
   const Weigher weigh(top, (double)temperature, sh.powers);
   const float reach = __fmul_rn(kReach, temperature), lowest = __fsub_rn(top, reach);  // below it weights vanish
-  const bool regular = __dmul_rn(fabs((double)top), weigh.rate) < 4398046511104.0;  // 2^42: near() holds
+  // near() holds: the largest logit's place below 2^42, and a temperature
+  // 2^46 times what widen() loses of a subnormal logit
+  const bool regular = __dmul_rn(fabs((double)top), weigh.rate) < 4398046511104.0 && temperature >= 8.2718061e-25f;
   const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0f, by_floor = min_p > 0.0f;
   const double floor_p = by_floor ? fmin((double)min_p, 1.0) : 0.0;
   const float share = fmaxf(top_p, 0.0f);

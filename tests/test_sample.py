@@ -354,3 +354,18 @@ def test_infinite_logits_at_an_infinite_temperature():
     tokens, probs = sample(torch.from_numpy(x.astype(np.float32)).cuda(), t, k, p, None, np.full(rows, 0.75))
     assert tokens.tolist() == [11, 500, 500, 11, 11, 500]
     assert probs.tolist() == [1.0, 0.5, 0.5, 1.0, 1.0, 0.5]
+
+
+@gpu
+def test_subnormal_logits_and_temperatures():
+    rng = np.random.default_rng(17)
+    rows, vocab = 12, 700
+    x = (rng.permuted(np.tile(np.arange(vocab), (rows, 1)), axis=1) * -1e-40).astype(np.float32)
+    t = np.full(rows, 2e-39, np.float32)
+    t[6:] = 3e-38
+    u = rng.random(rows)
+    check(x, t, None, None, None, u)
+    check(x, t, np.full(rows, 9), None, None, u)
+    check(x, t, None, np.full(rows, 0.7), None, u)
+    check(x, t, None, None, np.full(rows, 0.3), u)
+    assert status_bits() == 0
