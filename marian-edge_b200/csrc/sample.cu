@@ -116,27 +116,23 @@ struct Weigher {
   double top, rate;      // the weight's logit of 1; log2(e) / T
   uint32_t top_key;
   const double* powers;  // 2^-(j / 64)
-  double per_step, origin, per_logit, shift;
+  double per_step, per_logit;
 
   __device__ __forceinline__ Weigher(float top_, double temperature, const double* powers_)
-      : top((double)top_), rate(1.4426950408889634074 / temperature), top_key(key_of(top_)), powers(powers_) {
+      : top(widen(top_)), rate(1.4426950408889634074 / temperature), top_key(key_of(top_)), powers(powers_) {
     per_step = rate * -64.0;
-    origin = 6755399441055744.0 - per_step * top;  // 1.5 * 2^52 more: the sum is rounded to a whole number
     per_logit = 1.0 / temperature;
-    shift = -top * per_logit;
   }
-  // w = exp((v - top) / T): with k near 64 rate (top - v), 2^-(k / 64) from the
-  // table times exp(z), z = (v - top) / T + k ln 2 / 64, |z| <= 0.011, by its
-  // series to the fifth power (the sixth is below 3e-15).  For
-  // |top - v| rate < 1000 and |top| rate < 2^42, without a branch, so that
-  // several are in flight; above the top, w is above 1.  Returned as a
-  // product, *rest times the result.
+  // w = exp((v - top) / T) as *rest times the result: with k = 64 rate (top - v)
+  // to the nearest whole number (the sum with 1.5 * 2^52), 2^-(k / 64) from the
+  // table times exp(z), z = (v - top) / T + k ln 2 / 64, |z| <= 0.0055, by its
+  // series to the fourth power (the fifth is below 5e-14).  For |top - v| rate <
+  // 1000, without a branch, so that several are in flight; 1 at the top.
   __device__ __forceinline__ double near(float v, double* rest) const {
-    const double x = widen(v), t = __fma_rn(x, per_step, origin);
+    const double d = __dsub_rn(widen(v), top), t = __fma_rn(d, per_step, 6755399441055744.0);
     const int k = __double2loint(t);
-    const double z = __fma_rn(x, per_logit, __fma_rn(__dsub_rn(t, 6755399441055744.0), 0.010830424696249145, shift));
-    double s = __fma_rn(z, 1.0 / 120, 1.0 / 24);
-    s = __fma_rn(s, z, 1.0 / 6);
+    const double z = __fma_rn(__dsub_rn(t, 6755399441055744.0), 0.010830424696249145, __dmul_rn(d, per_logit));
+    double s = __fma_rn(z, 1.0 / 24, 1.0 / 6);
     s = __fma_rn(s, z, 0.5);
     s = __fma_rn(s, z, 1.0);
     *rest = __fma_rn(s, z, 1.0);
@@ -148,16 +144,22 @@ struct Weigher {
     const double p = near(v, &rest);
     return __dmul_rn(p, rest);
   }
+  __device__ __forceinline__ unsigned long long fixed_near(float v) const {
+    double rest;
+    const double p = near(v, &rest);
+    return last_bits(__fma_rn(p, rest, 4096.0));
+  }
   // Any v, top and T: 0 below 2^-42, 1 at the top even where it or rate is infinite.
   __device__ double real(float v, uint32_t key) const {
     if (key == top_key) return 1.0;
-    const double y = __dmul_rn(__dsub_rn(top, (double)v), rate);
+    const double y = __dmul_rn(__dsub_rn((double)value_of(top_key), (double)v), rate);
     return y < 42.0 ? exp2(-y) : 0.0;
   }
-  static __device__ __forceinline__ unsigned long long fixed(double w) {
-    // adding 2^12 leaves the 40 fraction bits at the end of the mantissa
-    return (unsigned long long)__double_as_longlong(__dadd_rn(w, 4096.0)) & ((1ull << 51) - 1);
+  // Of 2^12 + w: the 40 fraction bits are at the end of the mantissa.
+  static __device__ __forceinline__ unsigned long long last_bits(double w) {
+    return (unsigned long long)__double_as_longlong(w) & ((1ull << 51) - 1);
   }
+  static __device__ __forceinline__ unsigned long long fixed(double w) { return last_bits(__dadd_rn(w, 4096.0)); }
 };
 
 // What the CTAs of a row tell one another; two of each, used in turn, so
@@ -645,10 +647,8 @@ __device__ void finish_list(Row<T>& r, const Weigher& weigh, const Cuts& q, int 
     weight[j] = 0;
     if (first + j < in_a) {
       const uint32_t key = (uint32_t)(sh.list[first + j] >> 32);
-      const double real = weigh.near(value_of(key));
-      weight[j] = Weigher::fixed(real);
-      // the largest logit's weight is 1, from which near() may be a rounding off
-      above_floor += key == weigh.top_key || real >= q.floor_w;
+      weight[j] = weigh.fixed_near(value_of(key));
+      above_floor += weigh.near(value_of(key)) >= q.floor_w;
     }
     sum += weight[j];
   }
@@ -940,9 +940,9 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   }
   const Weigher weigh(top, (double)temperature, sh.powers);
   const float reach = __fmul_rn(kReach, temperature), lowest = __fsub_rn(top, reach);  // below it weights vanish
-  // near() holds: the largest logit's place below 2^42, and a temperature
-  // 2^46 times what widen() loses of a subnormal logit
-  const bool regular = __dmul_rn(fabs((double)top), weigh.rate) < 4398046511104.0 && temperature >= 8.2718061e-25f;
+  // near() holds: a temperature of 2^46 times what widen() loses of a subnormal
+  // logit or more, and numbers to subtract
+  const bool regular = top < INFINITY && temperature >= 8.2718061e-25f;
   const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0f, by_floor = min_p > 0.0f;
   const double floor_p = by_floor ? fmin((double)min_p, 1.0) : 0.0;
   const float share = fmaxf(top_p, 0.0f);
@@ -956,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
     if (by_p && !by_k) {
       r.each([&](float v, int) {
         const uint32_t b = bins.of(v);
-        const unsigned long long w = Weigher::fixed(weigh.near(v));
+        const unsigned long long w = weigh.fixed_near(v);
         if (b < kCoarse) {
           atomicAdd(&sh.counts[b], 1u);
           whole += w;
@@ -1013,7 +1013,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   const uint32_t key_min = top == INFINITY ? key_max : max(kKeyNone + 1, key_of(__fsub_rn(top, reach)));
   auto fixed_weight = [&](float v, uint32_t k) -> unsigned long long {
     if (!regular) return Weigher::fixed(weigh.real(v, k));
-    const unsigned long long w = Weigher::fixed(weigh.near(v));
+    const unsigned long long w = weigh.fixed_near(v);
     return v >= lowest ? w : 0ull;
   };
   Cut cut{kKeyNone, -1};

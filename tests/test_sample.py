@@ -369,3 +369,22 @@ def test_subnormal_logits_and_temperatures():
     check(x, t, None, np.full(rows, 0.7), None, u)
     check(x, t, None, None, np.full(rows, 0.3), u)
     assert status_bits() == 0
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["plain", "top_k", "top_p", "min_p"])
+def test_logits_far_from_zero(mode):
+    # neighbouring floats there, at temperatures of a few of their steps: the
+    # weights have to come from the differences
+    rng = np.random.default_rng(18)
+    rows, vocab = 24, 3000
+    offset = 2.0 ** rng.integers(4, 100, rows)
+    offset[0], offset[1:8] = 2.0 ** 127, -offset[1:8]
+    step = np.abs(offset) * 2.0 ** -22
+    x = offset[:, None] + step[:, None] * rng.integers(0, 200, (rows, vocab))
+    assert (x == x.astype(np.float32)).all()
+    arg = {"plain": {}, "top_k": {"k": rng.integers(1, 400, rows)}, "top_p": {"p": rng.uniform(0.1, 0.99, rows)},
+           "min_p": {"m": rng.uniform(0.01, 1.0, rows)}}[mode]
+    full = dict(t=step * rng.uniform(2.0, 20.0, rows), k=None, p=None, m=None, u=rng.random(rows))
+    check(x, **{**full, **arg})
+    assert status_bits() == 0
