@@ -98,8 +98,17 @@ __device__ __forceinline__ void mma_split(float (&d)[4], float (&rest)[4], const
   mma_tf32(d, ah, h0, h1);
 }
 
+// CTAs per SM that the registers are kept to, 0: as they come.  Ragged
+// sentences in 16 bits are latency, of which five CTAs hide more than four
+// (256 sentences, 8 heads of 64: 24.0 us, 25.0 with four, 41 with six, which
+// spill); f32 spills at four (14 us instead of 12 for 64 single tokens).
+template <typename T, int D>
+constexpr int small_blocks() {
+  return sizeof(T) == 2 && D <= 64 ? 5 : 0;
+}
+
 template <typename T, int D, int WR>
-__global__ void __launch_bounds__(128) cross_small_kernel(const CrossParams p) {
+__global__ void __launch_bounds__(128, small_blocks<T, D>()) cross_small_kernel(const CrossParams p) {
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int kType = kF32 ? MC_F32 : std::is_same<T, __half>::value ? MC_F16 : MC_BF16;
   constexpr int kKeys = Tile<T>::kKeys, kGroups = 4 / WR, kOwn = kKeys / kGroups, kNT = kOwn / 8;
