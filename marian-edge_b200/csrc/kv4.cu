@@ -350,9 +350,10 @@ __device__ __forceinline__ uint32_t high_codes(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ float half_exponent(uint32_t bits) {
-  const int e = (bits >> 10) & 31;
-  return (float)(e ? e - 15 : -24);
+// floor(log2 |v|) of an f16 value that is held in f32, where f16's subnormals
+// are normal; -24, the smallest one's, for 0.
+__device__ __forceinline__ float half_exponent(float v) {
+  return (float)max((int)((__float_as_uint(v) >> 23) & 255) - 127, -24);
 }
 
 template <int D, int NT, bool SPLIT>
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        ev[m][half] = half_exponent(vpair[m][half]);
+        ev[m][half] = half_exponent(unpack_f16(vpair[m][half]).x);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -683,3 +683,31 @@ def test_key_counts_next_to_the_largest_integer():
         att.max_kv_len = n
         assert lib.mc_kv4_attention_workspace(C.byref(cache), C.byref(att)) == 0
         assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == L.MC_INVALID_INPUT
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -17, 2.0 ** -15, 2.0 ** -13, 2.0 ** -11])
+def test_small_value_rows(dtype, size):
+    # scales around f16's smallest normal number, 2^-14, and far into its subnormals: a row's largest
+    # weight is taken with its scale and has to fit f16 all the same.  f16 outputs this small are
+    # multiples of 2^-24: 2^-25 more.
+    lib, rng = L.load(), np.random.default_rng(21)
+    lens = [1, 45, 700]
+    cache = Cache(3, 44, 16, 1, 64)
+    k, v = typed(rng, (sum(lens), 1, 64), "f32"), typed(rng, (sum(lens), 1, 64), "f32", size)
+    start = np.cumsum(lens) - lens
+    cs = cache.struct()
+    assert call(lib.mc_kv4_append, cs, rows_struct(k.cuda(), v.cuda(), start, lens, [0] * 3, 700, L.MC_F32)) == L.MC_OK
+    kd, vd = ((lambda c, s, m: m.astype(float)[..., None] + s.astype(float)[..., None] * c)(*quantize(f64(x))) for x in (k, v))
+    for q_size in (1.0, 20.0):
+        q = typed(rng, (3, 2, 64), dtype, q_size)
+        out, _, _ = attention(cache, q.cuda(), [0, 1, 2], [1] * 3, lens, 0.125, 0, dtype)
+        eps = torch.finfo(q.dtype).eps
+        for i, n in enumerate(lens):
+            ki, vi = kd[start[i]:start[i] + n], vd[start[i]:start[i] + n]
+            want, _ = attend(f64(q)[i:i + 1], ki, vi, 0.125, lambda j: n)
+            tol = (2.0 ** -18 if dtype == "f32" else eps / 2 + 2.0 ** -11) + 2 * score_error(f64(q)[i:i + 1], ki, 0.125)
+            np.testing.assert_allclose(f64(out)[i:i + 1], want, rtol=0,
+                                       atol=tol * np.abs(vi).max() + (2.0 ** -25 if dtype == "f16" else 0.0))
+    assert status_bits() == 0
