@@ -440,8 +440,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
       amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, o));
       sum = __fadd_rn(sum, __shfl_xor_sync(kFull, sum, o));
     }
-    // 2^(8 - exponent(amax)) as a bit pattern; tiny rows keep a finite factor.
-    const int e = min(max((int)((__float_as_uint(amax) >> 23) & 255) - 127, -110), 110);
+    // 2^(8 - exponent(amax)) as a bit pattern, for any finite amax; tiny rows
+    // keep a finite factor.
+    const int e = min(max((int)((__float_as_uint(amax) >> 23) & 255) - 127, -110), 127);
     const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
     const float down = __uint_as_float((uint32_t)(127 - 8 + e) << 23);
     auto part = [&](float a, float b2, float m) -> uint32_t {
@@ -603,7 +604,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
           float a = x[n][m][j];
           if (SPLIT) a = __fadd_rn(a, __shfl_xor_sync(kFull, a, 2));
           const float2 kp = j < 2 ? kp0 : kp1;
-          x[n][m][j] = __fmaf_rn(__fmul_rn(a, q_fac[n][j & 1]), kp.x, __fmul_rn(kp.y, q_sum[n][j & 1]));
+          // q's own size comes last: a code times it may pass the largest number
+          x[n][m][j] = __fmaf_rn(__fmul_rn(a, kp.x), q_fac[n][j & 1], __fmul_rn(kp.y, q_sum[n][j & 1]));
         }
       if (masked) {
 #pragma unroll

@@ -711,3 +711,24 @@ def test_small_value_rows(dtype, size):
             np.testing.assert_allclose(f64(out)[i:i + 1], want, rtol=0,
                                        atol=tol * np.abs(vi).max() + (2.0 ** -25 if dtype == "f16" else 0.0))
     assert status_bits() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("exponent", [110, 117, 118, 122, 126])
+def test_queries_up_to_the_largest_number(dtype, exponent):
+    # scores of 2^exponent are finite, and their weights one-hot: the output is one value row, to the
+    # type's rounding (f32: 2^-20, as the row's parts of up to 3 max|v| are within 2^-22 each).
+    # lse: 22-bit products (2^-21 of their sizes, of up to 3 max|k|).
+    rng = np.random.default_rng(exponent)
+    cache = Cache(1, 3, 16, 1, 64)
+    ks, vs = filled(rng, cache, [40])
+    q = torch.zeros(1, 2, 64)
+    q[0, 0, :3] = torch.tensor([1.0, -0.5, 0.75]) * 2.0 ** exponent
+    q[0, 1, 60:] = torch.tensor([-1.75, 0.0, 0.5, 1.5]) * 2.0 ** exponent
+    q = q.to(DTYPES[dtype][0])
+    out, lse, _ = attention(cache, q.cuda(), [0], [1], [40], 0.125, 0, dtype)
+    want, wl = attend(f64(q), ks[0], vs[0], 0.125, lambda j: 40)
+    tol = (2.0 ** -20 if dtype == "f32" else 2.0 ** -8 + 2.0 ** -11) * np.abs(vs[0]).max()
+    np.testing.assert_allclose(f64(out), want, rtol=0, atol=tol)
+    np.testing.assert_allclose(f64(lse), wl, rtol=0, atol=score_error(f64(q), ks[0], 0.125))
