@@ -732,3 +732,39 @@ def test_queries_up_to_the_largest_number(dtype, exponent):
     tol = (2.0 ** -20 if dtype == "f32" else 2.0 ** -8 + 2.0 ** -11) * np.abs(vs[0]).max()
     np.testing.assert_allclose(f64(out), want, rtol=0, atol=tol)
     np.testing.assert_allclose(f64(lse), wl, rtol=0, atol=score_error(f64(q), ks[0], 0.125))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,n,mean,spread,d,group", [
+    ("f32", 65536, 1.0, 0.1, 64, 1), ("f32", 65536, -1.0, 0.1, 48, 3), ("f32", 262144, 0.0, 1.0, 64, 1),
+    ("f32", 262144, 0.0, 1.0, 128, 8),
+    ("f16", 262144, 0.0, 1.0, 64, 1), ("bf16", 262144, 0.0, 1.0, 64, 1), ("f16", 262144, 0.0, 1.0, 80, 16)])
+def test_long_caches_of_many_sequences(dtype, n, mean, spread, d, group):
+    # So many sequences that no keys are cut into ranges: one warp sums them all.  Sums in f32 round to
+    # nearest, 2^-24.8 of the partial sum (root mean square) for each of n / 32 tiles, and for each of n / 8
+    # weights of eight lanes: 2^-19.3 of the whole at 65,536 keys and 2^-18.3 at 262,144.  f32 outputs:
+    # 2^-18 max|v| (root mean square), of values with a mean, whose sums grow with the keys.  16 bits, of
+    # values without one: the output's rounding, 2^-18 max|v| for the sums (which are 2^-6 of that size)
+    # and the weights' rounding, 2^-12.8 |v| / sqrt(n / 2.7) and so below 2^-20.
+    lib, b = L.load(), 1200
+    g = torch.Generator(device="cuda")
+    g.manual_seed(d)
+    one = Cache(1, n // 32, 32, 1, d, extra=0)
+    k, v = (torch.randn(n, 1, d, generator=g, device="cuda") for _ in range(2))
+    v = v * spread + mean
+    cs = one.struct()
+    assert call(lib.mc_kv4_append, cs, rows_struct(k, v, [0], [n], [0], n, L.MC_F32)) == L.MC_OK
+    assert call(lib.mc_kv4_read, cs, rows_struct(k, v, [0], [n], [0], n, L.MC_F32)) == L.MC_OK
+    one.b, one.table_dev = b, one.table_dev.expand(b, n // 32).contiguous()   # every sequence reads the same pages
+    q = torch.randn(b, group, d, generator=g, device="cuda").to(DTYPES[dtype][0])
+    out, lse, need = attention(one, q, np.arange(b), [1] * b, [n] * b, d ** -0.5, 0, dtype)
+    assert need == 0 and status_bits() == 0
+    at = [0, 1, b // 2, b - 1]
+    x = q[at].double().reshape(-1, d) @ k[:, 0].double().T * d ** -0.5
+    want = torch.softmax(x, 1) @ v[:, 0].double()
+    got, big = out[at].double().reshape(-1, d), float(v.abs().max())
+    if dtype == "f32":
+        assert float((got - want).square().mean().sqrt()) <= 2.0 ** -18 * big
+    else:
+        assert bool(((got - want).abs() <= torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -18 * big).all())
+    np.testing.assert_allclose(lse[at].double().reshape(-1).cpu(), torch.logsumexp(x, 1).cpu(), rtol=2.0 ** -18)
