@@ -429,7 +429,9 @@ mc_status mc_kv4_attention(const mc_kv4_cache *cache, const mc_kv4_attention_arg
  * zeros and lse -inf; lse (nullable, [q_rows][heads]) receives ln sum_j w_j.
  * Rows outside every sequence are left as they were; q ranges must not
  * overlap.  16-bit types: the weights are rounded to the type before they
- * meet the values; f32: products to 2^-21. */
+ * meet the values; f32: products to 2^-21.  Infinities and NaN go the way of
+ * f32 arithmetic: a key whose score is -inf has a weight of 0, an infinite
+ * value gives an infinite output. */
 typedef struct {
     const void *q, *k, *v;       /* 16-byte aligned; strides * element size multiples of 16 */
     void *out;                   /* may not overlap q, k or v */

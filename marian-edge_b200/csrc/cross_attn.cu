@@ -444,6 +444,98 @@ __global__ void __launch_bounds__(128, small_blocks<T, D>()) cross_small_kernel(
         part[16 * D + g + 8 * h] = lse2[h];
     }
   }
+  if constexpr (kF32) {
+    // A value that rounds past the largest number, or an infinity, has no two
+    // tf32 halves (its low part is an infinity or a NaN), and shifted weights
+    // times values next to the largest may pass it: a row that is not finite
+    // is computed again from its f32 numbers, key after key, a pair of
+    // channels per lane.
+    uint32_t lost[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bool finite = fabsf(sum[h]) < INFINITY;
+#pragma unroll
+      for (int i = 0; i < kOut; ++i) finite = finite && fabsf(acc[i][2 * h]) < INFINITY && fabsf(acc[i][2 * h + 1]) < INFINITY;
+      lost[h] = __ballot_sync(kFull, !finite);
+    }
+    if (lost[0] | lost[1]) {
+      __syncwarp();
+#pragma unroll 1
+      for (int own_row = 0; own_row < 16; ++own_row) {
+        const int row = wr * 16 + own_row;
+        if (row0 + row >= n_rows) break;
+        if (!((own_row < 8 ? lost[0] : lost[1]) >> (4 * (own_row & 7)) & 15)) continue;
+        constexpr int kPairs = (D + 63) / 64;
+        const int pos = (int)share((uint32_t)(row0 + row), (uint32_t)r.group), qh = head * r.group + (row0 + row) - pos * r.group;
+        const float* q = static_cast<const float*>(r.q) + (long long)(seq.q0 + pos) * r.q_row_stride + (long long)qh * r.q_head_stride;
+        float2 qv[kPairs], o[kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          const int ch = 64 * i + 2 * lane;
+          qv[i] = ch < D ? *reinterpret_cast<const float2*>(q + ch) : make_float2(0.0f, 0.0f);
+          o[i] = make_float2(0.0f, 0.0f);
+        }
+        // a NaN in the query leaves nothing to compute
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) nan = nan || qv[i].x != qv[i].x || qv[i].y != qv[i].y;
+        if (__any_sync(kFull, nan)) continue;
+        float most = -INFINITY, total = 0.0f;
+#pragma unroll 1
+        for (int at = 0; at < (end - begin) * kOwn; ++at) {
+          const int key = (begin + at / kOwn) * kKeys + kg * kOwn + at % kOwn;
+          if (key >= seq.nk || (mask && !mask[key])) continue;
+          float2 v[kPairs];
+          float x = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const int ch = 64 * i + 2 * lane;
+            v[i] = make_float2(0.0f, 0.0f);
+            if (ch < D) {
+              const float2 k2 = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(kbase) + (long long)key * p.k_rs + ch);
+              v[i] = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(vbase) + (long long)key * p.v_rs + ch);
+              x = __fmaf_rn(qv[i].y, k2.y, __fmaf_rn(qv[i].x, k2.x, x));
+            }
+          }
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) x = __fadd_rn(x, __shfl_xor_sync(kFull, x, d));
+          x = __fmul_rn(x, factor);
+          if (x > most) {
+            const float shrink = most == -INFINITY ? 0.0f : exp2_approx(__fsub_rn(most, x));
+            most = x;
+            total = __fmul_rn(total, shrink);
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) o[i] = make_float2(__fmul_rn(o[i].x, shrink), __fmul_rn(o[i].y, shrink));
+          }
+          const float w = x == -INFINITY ? 0.0f : exp2_approx(__fsub_rn(x, most));
+          total = __fadd_rn(total, w);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) o[i] = make_float2(__fmaf_rn(w, v[i].x, o[i].x), __fmaf_rn(w, v[i].y, o[i].y));
+        }
+        const float share_of = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+        const float l = total == 0.0f ? -INFINITY : __fadd_rn(most, log2f(total));
+        const Place to = kGroups == 1 ? place_of(row) : Place{};
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          const int ch = 64 * i + 2 * lane;
+          if (ch >= D) continue;
+          const float a = __fmul_rn(o[i].x, share_of), c = __fmul_rn(o[i].y, share_of);
+          if (kGroups == 1) {
+            emit(to, ch, a, c);
+          } else {
+            part[own_row * D + ch] = a;
+            part[own_row * D + ch + 1] = c;
+          }
+        }
+        if (lane == 0) {
+          if (kGroups == 1)
+            emit_lse(to, l);
+          else
+            part[16 * D + own_row] = l;
+        }
+      }
+    }
+  }
   if (kGroups == 1) return;
   __syncthreads();
   // ---- join the key groups: warp w takes every fourth row ----

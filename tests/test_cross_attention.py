@@ -394,3 +394,63 @@ def test_key_counts_next_to_the_largest_integer():
         a.k_rows = a.max_k_len = n
         assert lib.mc_cross_attention_workspace(C.byref(a)) == 0
         assert lib.mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
+
+
+@gpu
+@pytest.mark.parametrize("d,q_len,n", [(64, 1, 90), (48, 20, 90), (128, 70, 90), (64, 1, 3000), (16, 2, 33)])
+@pytest.mark.parametrize("case", ["k lowest", "k -inf", "v inf", "v -inf", "v largest", "v all large", "q largest", "k inf"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_f32_infinities_and_largest_numbers(d, q_len, n, case, masked):
+    # 64-bit arithmetic says what comes of them: a score of -inf (or far below the others) is a weight of 0,
+    # an infinite value an infinite output, and a NaN only what has none.  Tolerances as in compare(), per
+    # channel, since one channel may hold numbers of another size.
+    rng = np.random.default_rng(d + n)
+    q, k, v = (typed(rng, (m, 2, d), "f32") for m in (q_len, n, n))
+    q = q.abs() + 0.1
+    mask = None
+    if masked:
+        mask = (rng.random(n) < 0.7).astype(np.uint8)
+        mask[5], mask[7] = 1, 0
+        k[7], v[7] = float("inf"), float("nan")     # left out
+    big = 3.4028234663852886e38
+    if case == "k lowest":
+        k[5, 0] = -big
+    elif case == "k -inf":
+        k[5, 0, 3] = -float("inf")
+    elif case == "k inf":
+        k[5, 0, 3] = float("inf")
+    elif case == "v inf":
+        v[5, 0, 3] = float("inf")
+    elif case == "v -inf":
+        v[5, 0, 2], v[5, 0, 3], v[2, 0, 3] = -float("inf"), -float("inf"), float("inf")
+        if masked:
+            mask[2] = 1
+    elif case == "v largest":
+        v[5, 0, 3], v[5, 0, 4] = big, -big
+    elif case == "v all large":                     # sums of at most 3,000 weights of 1 stay in range
+        v[:, 0, 3] = torch.from_numpy(rng.uniform(-1e34, 1e34, n).astype(np.float32))
+    else:
+        q[0, 0, 3] = big
+        k[:, 0, 3] = torch.from_numpy(rng.uniform(-1e-38, 1e-38, n).astype(np.float32))
+    scale = d ** -0.5
+    out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), [0], [q_len], [0], [n], "f32", scale, mask)
+    live = np.ones(n, bool) if mask is None else mask != 0
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, wl = attend(f64(q), f64(k), f64(v), scale, live)
+    got, finite_v = f64(out), np.where(np.isfinite(f64(v)), f64(v), 0.0)[live]
+    small_k = np.where(np.abs(f64(k)) < 1e30, f64(k), 0.0)[live]
+    small_q = np.where(np.abs(f64(q)) < 1e30, f64(q), 3.4)      # its products with k are at most that
+    dx = 2.0 ** -20 * scale * np.abs(small_q).sum(-1).max() * max(1.0, np.abs(small_k).max())
+    if case == "k inf":
+        assert np.isnan(got[:, 0]).all() and np.isnan(f64(lse)[:, 0]).all()
+        got, want, wl, lse = got[:, 1:], want[:, 1:], wl[:, 1:], lse[:, 1:]
+        finite_v = finite_v[:, 1:]
+    assert (np.isnan(got) == np.isnan(want)).all() and (np.isinf(got) == np.isinf(want)).all()
+    for j in range(got.shape[1]):
+        for c in range(d):
+            w, g = want[:, j, c], got[:, j, c]
+            some = np.isfinite(w)
+            assert (g[np.isinf(w)] == w[np.isinf(w)]).all()
+            np.testing.assert_allclose(g[some], w[some], rtol=0, atol=(2.0 ** -18 + 2 * dx) * np.abs(finite_v[:, j, c]).max())
+    np.testing.assert_allclose(f64(lse), wl, rtol=2.0 ** -20, atol=2.0 ** -19 + dx)
+    assert status_bits() == 0
