@@ -10,7 +10,8 @@
 // 4-7 and 8-11 hold one query row per thread of tile 0 and 1: they read S_i,
 // keep the row's maximum and sum, and write the weights, rounded to the
 // type, over S_i.  O_i is only rescaled when a maximum grows by more than 8
-// (in powers of two): the weights stay below 2^8, and their sum is as stale.
+// (in powers of two): the weights stay below 2^8 (f16: 2^15, by weight_shift),
+// and their sum is as stale.
 //
 // What bounds it: with M = N = 128 the tensor pipe, one issuing warp's round
 // through its barriers between the products of a step, and the exponentials
@@ -35,6 +36,11 @@ constexpr uint32_t kFull = 0xFFFFFFFFu;
 constexpr int kThreads = 384;
 constexpr int kTileBytes = 128 * 128;  // 128 rows of 64 channels
 constexpr float kGrowth = 8.0f;
+// f16 weights are taken 2^7 larger, so that those down to 2^-21 of a row's
+// maximum are normal numbers and only those below 2^-32 are lost: in a long tail
+// behind one key they count together.  With the growth they stay below 2^15.
+// bf16 has f32's range.
+constexpr float weight_shift(bool bf16) { return bf16 ? 0.0f : 7.0f; }
 
 constexpr int chunks_of(int d) { return (d + 63) / 64; }
 // Ring stages, each for the V tile of one step and the K tile of the next,
@@ -139,6 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     cross_long_kernel(const CrossParams p, const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map) {
   constexpr int kChunks = chunks_of(D), kStages = stages_of(D), kSteps = D / 16;
+  constexpr float kShift = weight_shift(BF16);
   constexpr uint32_t kS0 = 0, kO0 = 256;  // TMEM columns: S_i at 128 i, O_i at 256 + 128 i
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      const float base = top == -INFINITY ? 0.0f : __fmul_rn(-top, factor);
+      const float base = top == -INFINITY ? 0.0f : BF16 ? __fmul_rn(-top, factor) : __fmaf_rn(-top, factor, kShift);
       const uint64_t factor2 = pair(factor, factor), base2 = pair(base, base);
       uint64_t add[2] = {0, 0};
 #pragma unroll
@@ -402,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool written = i < row_tiles && ok && there;
     // ---- the row, normalized ----
     const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-    const float lse2 = sum == 0.0f ? -INFINITY : __fadd_rn(__fmul_rn(top, factor), log2f(sum));
+    const float lse2 = sum == 0.0f ? -INFINITY : __fadd_rn(BF16 ? __fmul_rn(top, factor) : __fmaf_rn(top, factor, -kShift), log2f(sum));
     const bool direct = parts <= 1;
     const long long slot = ((long long)nth * kLongRows + 128 * i + row_in) * p.split.splits + split;
     __syncwarp();

@@ -454,3 +454,37 @@ def test_f32_infinities_and_largest_numbers(d, q_len, n, case, masked):
             np.testing.assert_allclose(g[some], w[some], rtol=0, atol=(2.0 ** -18 + 2 * dx) * np.abs(finite_v[:, j, c]).max())
     np.testing.assert_allclose(f64(lse), wl, rtol=2.0 ** -20, atol=2.0 ** -19 + dx)
     assert status_bits() == 0
+
+
+def long_tail(dtype, b, nats, at, masked):
+    """One key `nats` above 65,535 equal ones: each of those has a weight of some 2^-25 of the largest, all
+    of them together count.  With 148 sequences no keys are cut into ranges.  16-bit weights are rounded to
+    the type, and in f16 to 2^-24 at 2^7 (long tiles) or more times their size: 2^-32 of the largest.  Tiles of
+    64 keys or more are added up in f32: at most 2^10 roundings of 2^-24 of the sum each, of which the key
+    that stands out, whose value is 0, has no part in the output's numerator."""
+    rng, n, m = np.random.default_rng(at), 65536, 128
+    q, k = torch.zeros(m * b, 1, 64), torch.zeros(n, 1, 64)
+    q[:, 0, 0], k[at, 0, 0] = 8.0, nats
+    v = torch.from_numpy(rng.uniform(0.5, 1.5, (n, 1, 64)).astype(np.float32))
+    v[at] = 0.0
+    q, k, v = (x.to(DTYPES[dtype][0]) for x in (q, k, v))
+    out, lse, need = run(q.cuda(), k.cuda(), v.cuda(), np.arange(b) * m, [m] * b, [0] * b, [n] * b, dtype, 0.125,
+                         np.ones(n, np.uint8) if masked else None)
+    w = np.exp(f64(k)[:, 0, 0] - f64(k)[at, 0, 0])
+    want = w @ f64(v)[:, 0] / w.sum()
+    tol = (torch.finfo(q.dtype).eps + 2.0 ** -13) * want + (n * 2.0 ** -32 * 1.5 if dtype == "f16" else 0.0)
+    got = out.double().reshape(m * b, 64).cpu().numpy()
+    assert (np.abs(got - want) <= tol).all(), np.abs(got - want).max()
+    np.testing.assert_allclose(f64(lse), f64(k)[at, 0, 0] + np.log(w.sum()), rtol=2.0 ** -20, atol=2.0 ** -14)
+    assert status_bits() == 0
+
+
+LONG_TAILS = [(148, 17.4, 0), (148, 17.4, 40000), (148, 17.4, 65535), (148, 19.0, 100), (148, 5.5, 200),
+              (148, 5.5, 65000), (1, 17.4, 30000)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("b,nats,at", LONG_TAILS)
+def test_a_long_tail_behind_one_key(dtype, b, nats, at):
+    long_tail(dtype, b, nats, at, False)
