@@ -308,13 +308,16 @@ __global__ void __launch_bounds__(128, small_blocks<T, D>()) cross_small_kernel(
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) base[h] = top[h] == -INFINITY ? 0.0f : __fsub_rn(top[h], kShift);
+      float here[2] = {0.0f, 0.0f};  // small weights are added up before they meet a large sum
 #pragma unroll
       for (int j = 0; j < kNT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[j][e] = exp2_approx(__fsub_rn(x[j][e], base[e >> 1]));
-          sum[e >> 1] = __fadd_rn(sum[e >> 1], x[j][e]);
+          here[e >> 1] = __fadd_rn(here[e >> 1], x[j][e]);
         }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sum[h] = __fadd_rn(sum[h], here[h]);
       // ---- values ----
       if constexpr (kF32) {
         // k = t: column 2 t (key t); k = t + 4: column 2 t + 1 (key t + 4)

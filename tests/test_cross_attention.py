@@ -488,3 +488,10 @@ LONG_TAILS = [(148, 17.4, 0), (148, 17.4, 40000), (148, 17.4, 65535), (148, 19.0
 @pytest.mark.parametrize("b,nats,at", LONG_TAILS)
 def test_a_long_tail_behind_one_key(dtype, b, nats, at):
     long_tail(dtype, b, nats, at, False)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("b,nats,at", LONG_TAILS)
+def test_a_long_tail_behind_one_key_with_a_mask(dtype, b, nats, at):
+    long_tail(dtype, b, nats, at, True)
