@@ -667,6 +667,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
       float base[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) base[j] = top[n][j] == -INFINITY ? 0.0f : __fsub_rn(top[n][j], 10.0f);
+      float here_p[2] = {0.0f, 0.0f}, here_m[2] = {0.0f, 0.0f};  // small weights are added up before they meet a large sum
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -677,8 +678,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float e = exp2_approx(__fsub_rn(x[n][m][2 * half + j], base[j]));
-            sum_p[n][j] = __fadd_rn(sum_p[n][j], e);
-            sum_m[n][j] = __fmaf_rn(e, vp.y, sum_m[n][j]);
+            here_p[j] = __fadd_rn(here_p[j], e);
+            here_m[j] = __fmaf_rn(e, vp.y, here_m[j]);
             w[j] = __fmul_rn(e, vp.x);
           }
           uint32_t packed = pack_f16(w[0], w[1]);
@@ -690,6 +691,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks(NT)) kv4_attn_ker
           }
           wb[n][m][half] = transpose8(packed);
         }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        sum_p[n][j] = __fadd_rn(sum_p[n][j], here_p[j]);
+        sum_m[n][j] = __fadd_rn(sum_m[n][j], here_m[j]);
+      }
     }
 
     // ---- values: byte i of a lane holds channels 2c (row g) and 2c + 1 (row g + 8) ----

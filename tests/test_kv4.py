@@ -768,3 +768,33 @@ def test_long_caches_of_many_sequences(dtype, n, mean, spread, d, group):
     else:
         assert bool(((got - want).abs() <= torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -18 * big).all())
     np.testing.assert_allclose(lse[at].double().reshape(-1).cpu(), torch.logsumexp(x, 1).cpu(), rtol=2.0 ** -18)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nats,at", [(17.4, 0), (17.4, 40000), (16.0, 9), (5.5, 200)])
+def test_a_long_tail_behind_one_key(dtype, nats, at):
+    # One key `nats` above 65,535 equal ones, whose weights count together; so many sequences that one warp
+    # sums them all.  A lane adds up its four weights of a tile before they meet its sum: 2^11 roundings of
+    # 2^-24 of the largest weight, which is nearly the whole sum, in one of eight lanes.  The key that stands
+    # out has the value 0, so the output is as far off as the sum, and its type's rounding.
+    lib, b, n, d = L.load(), 1200, 65536, 64
+    rng = np.random.default_rng(at)
+    one = Cache(1, n // 32, 32, 1, d, extra=0)
+    k = torch.zeros(n, 1, d, device="cuda")
+    k[at, 0, 0] = nats
+    v = torch.from_numpy(rng.uniform(0.5, 1.5, (n, 1, d)).astype(np.float32)).cuda()
+    v[at] = 0.0
+    cs = one.struct()
+    assert call(lib.mc_kv4_append, cs, rows_struct(k, v, [0], [n], [0], n, L.MC_F32)) == L.MC_OK
+    assert call(lib.mc_kv4_read, cs, rows_struct(k, v, [0], [n], [0], n, L.MC_F32)) == L.MC_OK
+    one.b, one.table_dev = b, one.table_dev.expand(b, n // 32).contiguous()
+    q = torch.zeros(b, 1, d, dtype=DTYPES[dtype][0], device="cuda")
+    q[:, 0, 0] = 8.0
+    out, lse, need = attention(one, q, np.arange(b), [1] * b, [n] * b, 0.125, 0, dtype)
+    assert need == 0 and status_bits() == 0
+    x = k[:, 0, 0].double()
+    want = torch.softmax(x, 0) @ v[:, 0].double()
+    rounding = 2.0 ** -18 if dtype == "f32" else torch.finfo(q.dtype).eps / 2 + 2.0 ** -11
+    assert bool(((out[:, 0].double() - want).abs() <= (2.0 ** -13 + rounding) * want).all())
+    np.testing.assert_allclose(f64(lse), float(torch.logsumexp(x, 0)), rtol=2.0 ** -20, atol=2.0 ** -13)
