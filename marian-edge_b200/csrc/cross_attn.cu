@@ -590,10 +590,22 @@ bool cross_sizes_ok(const mc_cross_attention_args* a) {
 
 // Long tiles pay where the sequences' rows fill one of two on average: below,
 // the small kernel's 16-row warps waste less.
+bool long_fits(const mc_cross_attention_args* a, int64_t positions) {
+  return a->dtype != MC_F32 && a->heads / a->kv_heads * positions >= kLongRows / 2 && a->max_k_len >= kLongKeys;
+}
 bool long_pays(const mc_cross_attention_args* a) {
-  const int64_t mean = a->batch > 0 ? a->q_rows / a->batch : 0, group = a->heads / a->kv_heads;
-  return a->dtype != MC_F32 && !a->key_mask && a->scale > 0.0f && cross_long_strides(a) &&
-         group * (mean < a->max_q_len ? mean : a->max_q_len) >= 128 && a->max_k_len >= 128;
+  const int64_t mean = a->batch > 0 ? a->q_rows / a->batch : 0;
+  return !a->key_mask && a->scale > 0.0f && cross_long_strides(a) && long_fits(a, mean < a->max_q_len ? mean : a->max_q_len);
+}
+
+// The most keys that one CTA sums.  In 16 bits a row's sum over its keys stays
+// in the tensor cores' accumulator, whose additions cut off up to 2^-23 of it,
+// once for 16 keys: 2^-13 of the output over 2^14 keys (f16) and 2^-10 over 2^17
+// (bf16), a quarter of half a step of the type.  (f16, 262,144 keys of one sign in
+// one range: 2e-3 too small.  Sums per tile in registers, as f32 has, cost the
+// small tiles 20% at 2 x 1,024 x 2,048 and 5% on ragged sentences.)
+int64_t most_keys(int32_t dtype) {
+  return dtype == MC_F16 ? 1 << 14 : dtype == MC_BF16 ? 1 << 17 : INT32_MAX;
 }
 
 CrossPlan cross_plan(const mc_cross_attention_args* a, bool long_tiles) {
@@ -619,7 +631,11 @@ CrossPlan cross_plan(const mc_cross_attention_args* a, bool long_tiles) {
   }
   long long splits = cut > 0 ? kSms * (long_tiles ? 1 : 3) / cut : 1;
   if (splits > tiles / 4) splits = tiles / 4;
+  const long long needed = (a->max_k_len + most_keys(a->dtype) - 1) / most_keys(a->dtype);
+  if (needed > 1) plan.first = 0;  // no unit is whole
+  if (splits < needed) splits = needed;
   if (splits > 256) splits = 256;
+  if (plan.units > 0 && splits > INT32_MAX / plan.units) splits = INT32_MAX / plan.units;
   if (splits < 1) splits = 1;
   plan.chunk = tiles > 0 ? (int)((tiles + splits - 1) / splits) : 1;
   plan.splits = tiles > 0 ? (tiles + plan.chunk - 1) / plan.chunk : 1;
@@ -685,9 +701,9 @@ cudaError_t launch_cross(CrossParams p, const CrossPlan& plan, void* workspace, 
 
 extern "C" uint64_t mc_cross_attention_workspace(const mc_cross_attention_args* args) {
   if (!mc::cross_sizes_ok(args)) return 0;
-  // either kernel may run: which one also goes by the strides and the mask
+  // where both may run, which one goes by the strides, the mask and the rows in use
   const uint64_t small = mc::cross_plan(args, false).bytes;
-  const uint64_t wide = args->dtype == MC_F32 ? 0 : mc::cross_plan(args, true).bytes;
+  const uint64_t wide = mc::long_fits(args, args->max_q_len) ? mc::cross_plan(args, true).bytes : 0;
   return small > wide ? small : wide;
 }
 

@@ -495,3 +495,47 @@ def test_a_long_tail_behind_one_key(dtype, b, nats, at):
 @pytest.mark.parametrize("b,nats,at", LONG_TAILS)
 def test_a_long_tail_behind_one_key_with_a_mask(dtype, b, nats, at):
     long_tail(dtype, b, nats, at, True)
+
+
+@gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype,b,m,n,d", [
+    ("f16", 460, 1, 262144, 64), ("f16", 460, 20, 262144, 48), ("f16", 148, 128, 262144, 64),
+    ("f16", 150, 130, 100001, 128), ("bf16", 460, 1, 1048576, 64), ("bf16", 148, 128, 1048576, 64)])
+def test_many_keys_of_one_sign(dtype, b, m, n, d, masked):
+    # Equal weights, which are exact, over so many sequences that they fill the GPU: what is left is half a
+    # step of the output, 2^-11 (f16) or 2^-8 for 1 to 2, and what the tensor cores' additions cut off, 2^-23
+    # for each 16 keys of a range: 2^-13 of the output in 2^14 keys (f16), 2^-10 in 2^17 (bf16).
+    g = torch.Generator(device="cuda")
+    g.manual_seed(d)
+    q = torch.zeros(b * m, 1, d, dtype=DTYPES[dtype][0], device="cuda")
+    k = torch.randn(n, 1, d, generator=g, device="cuda").to(q.dtype)
+    v = (torch.rand(n, 1, d, generator=g, device="cuda") * 0.8 + 1.0).to(q.dtype)
+    k_len = np.full(b, n)
+    k_len[1], k_len[3] = 40, 0          # sequences of one range and of none
+    out, lse, need = run(q, k, v, np.arange(b) * m, [m] * b, [0] * b, k_len, dtype, d ** -0.5,
+                         np.ones(n, np.uint8) if masked else None)
+    assert need > 0 and status_bits() == 0
+    want = torch.stack([v[:x, 0].double().mean(0) if x else torch.zeros(d, device="cuda", dtype=torch.float64) for x in k_len[:4]])
+    want = want[torch.arange(b, device="cuda").clamp(max=4) % 4].repeat_interleave(m, 0)
+    error = (out.double()[:, 0] - want).abs()
+    share = 2.0 ** -13 if dtype == "f16" else 2.0 ** -10
+    assert bool((error <= (2.0 ** -11 if dtype == "f16" else 2.0 ** -8) + share * want).all()), float(error.max())
+    np.testing.assert_allclose(f64(lse)[:m], np.log(n), rtol=0, atol=2.0 ** -17)
+    np.testing.assert_allclose(f64(lse)[-m:], np.log(n), rtol=0, atol=2.0 ** -17)
+    assert np.isneginf(f64(lse)[3 * m:4 * m]).all()
+
+
+def test_ranges_of_16_bit_keys_are_bounded():
+    # the workspace follows the number of ranges: 512 units of 64 rows (small tiles) fill the GPU
+    lib, a = L.load(), host_args()
+    a.batch, a.heads, a.kv_heads, a.max_q_len, a.key_mask = 64, 8, 8, 64, 64
+    slots = 64 * 8 * 64
+    for dtype, most in ((L.MC_F32, None), (L.MC_F16, 1 << 14), (L.MC_BF16, 1 << 17)):
+        a.dtype = dtype
+        for n in (1, 1 << 14, (1 << 14) + 1, 1 << 17, (1 << 17) + 1, 1 << 20):
+            a.max_k_len = a.k_rows = n
+            ranges = 1 if most is None else -(-n // most)
+            least = 0 if ranges == 1 else slots * ranges * (64 + 1) * 4
+            got = lib.mc_cross_attention_workspace(C.byref(a))
+            assert got >= least and (dtype != L.MC_F32 or got == 0)
