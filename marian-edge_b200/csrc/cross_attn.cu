@@ -585,6 +585,7 @@ bool cross_sizes_ok(const mc_cross_attention_args* a) {
          a->heads % a->kv_heads == 0 && a->head_dim >= 16 && a->head_dim <= kOpMaxHeadDim && a->head_dim % 16 == 0 &&
          a->max_q_len >= 0 && a->max_k_len >= 0 && a->max_k_len <= kOpMaxKeys && a->heads <= 65536 &&
          (int64_t)(a->heads / a->kv_heads) * a->max_q_len <= INT32_MAX / 2 &&
+         (int64_t)a->batch * a->kv_heads <= INT32_MAX &&  // the product below stays within 64 bits
          (int64_t)a->batch * a->kv_heads * ((int64_t)(a->heads / a->kv_heads) * a->max_q_len / 16 + 1) <= INT32_MAX;
 }
 

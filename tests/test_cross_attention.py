@@ -539,3 +539,14 @@ def test_ranges_of_16_bit_keys_are_bounded():
             least = 0 if ranges == 1 else slots * ranges * (64 + 1) * 4
             got = lib.mc_cross_attention_workspace(C.byref(a))
             assert got >= least and (dtype != L.MC_F32 or got == 0)
+
+
+def test_products_of_sizes_past_64_bits_are_refused():
+    # 2^30 sequences x 2^16 heads x row tiles of 16 rows: (2^28 / 16 + 1) * 2^46 is past 2^63, and what a
+    # 64-bit product keeps of it looks small
+    lib = L.load()
+    for batch, heads, max_q_len in ((2**30, 65536, 2**22 - 16), (2**30, 65536, 2**30 - 16), (2**16, 2**16, 1), (2**31 - 1, 2, 1)):
+        a = host_args()
+        a.batch, a.heads, a.kv_heads, a.max_q_len, a.q_rows = batch, heads, heads, max_q_len, 1
+        assert lib.mc_cross_attention_workspace(C.byref(a)) == 0
+        assert lib.mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
