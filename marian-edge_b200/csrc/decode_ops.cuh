@@ -203,19 +203,22 @@ inline mc_status launched(cudaError_t e) {
 }
 
 // Rows of head_dim values whose strides keep every 16-byte load aligned.
+constexpr int64_t kOpMaxStride = int64_t(1) << 40;
 inline bool strides_ok(const void* base, int64_t row_stride, int64_t head_stride, int bytes) {
-  return base && aligned16(base) && row_stride >= 0 && head_stride >= 0 && (row_stride * bytes) % 16 == 0 &&
-         (head_stride * bytes) % 16 == 0 && row_stride < (int64_t(1) << 40) && head_stride < (int64_t(1) << 40);
+  return base && aligned16(base) && row_stride >= 0 && head_stride >= 0 && row_stride < kOpMaxStride &&
+         head_stride < kOpMaxStride && (row_stride * bytes) % 16 == 0 && (head_stride * bytes) % 16 == 0;
 }
 
 // Written rows must not overlap each other: either the heads of a row lie
-// within the row's stride, or the rows of a head within the head's.
+// within the row's stride, or the rows of a head within the head's.  (2^31 rows
+// or heads times a stride pass 64 bits.)
 inline bool strides_apart(int64_t rows, int64_t heads, int64_t head_dim, int64_t row_stride, int64_t head_stride) {
   const bool head_ok = heads <= 1 || head_stride >= head_dim;
   const bool row_ok = rows <= 1 || row_stride >= head_dim;
   if (!head_ok || !row_ok) return false;
   if (rows <= 1 || heads <= 1) return true;
-  return row_stride >= (heads - 1) * head_stride + head_dim || head_stride >= (rows - 1) * row_stride + head_dim;
+  return row_stride >= static_cast<__int128>(heads - 1) * head_stride + head_dim ||
+         head_stride >= static_cast<__int128>(rows - 1) * row_stride + head_dim;
 }
 
 // Raises a kernel's dynamic shared memory limit, once per device.

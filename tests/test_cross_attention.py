@@ -550,3 +550,15 @@ def test_products_of_sizes_past_64_bits_are_refused():
         a.batch, a.heads, a.kv_heads, a.max_q_len, a.q_rows = batch, heads, heads, max_q_len, 1
         assert lib.mc_cross_attention_workspace(C.byref(a)) == 0
         assert lib.mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
+
+
+def test_overlaps_of_wide_strides_are_refused():
+    # (rows - 1) * row_stride passes 64 bits, and what is left of it looks small: head 2^15 of a row would be
+    # head 0 of the next
+    a = host_args()
+    a.batch, a.heads, a.kv_heads, a.max_q_len, a.q_rows = 1, 65536, 65536, 1, 2**30 + 1
+    a.out_row_stride, a.out_head_stride = 2**34, 2**19
+    assert L.load().mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
+    a.out_head_stride = 2**18
+    sound = L.MC_INVALID_INPUT if torch.cuda.is_available() else L.MC_CUDA   # past the checks; there is no such memory
+    assert L.load().mc_cross_attention(C.byref(a), None) == sound

@@ -798,3 +798,32 @@ def test_a_long_tail_behind_one_key(dtype, nats, at):
     rounding = 2.0 ** -18 if dtype == "f32" else torch.finfo(q.dtype).eps / 2 + 2.0 ** -11
     assert bool(((out[:, 0].double() - want).abs() <= (2.0 ** -13 + rounding) * want).all())
     np.testing.assert_allclose(f64(lse), float(torch.logsumexp(x, 0)), rtol=2.0 ** -20, atol=2.0 ** -13)
+
+
+def test_overlaps_of_wide_strides_are_refused():
+    # (rows - 1) * row_stride or (heads - 1) * head_stride pass 64 bits, and what is left of them looks small
+    lib = L.load()
+    sound = L.MC_INVALID_INPUT if torch.cuda.is_available() else L.MC_CUDA   # past the checks; there is no such memory
+    for rows, heads, row_stride, head_stride, want in (
+            (2**30 + 1, 65536, 2**34, 2**19, L.MC_INVALID_INPUT),   # head 2^15 of a row is head 0 of the next
+            (2**30 + 1, 65536, 2**34, 2**18, sound),                # 65,536 heads within the row's stride
+            (2**30 + 1, 4, 2**34, 64, sound)):
+        cache, r, att = host_args()
+        cache.batch, cache.kv_heads = 1, heads
+        att.heads, att.q_rows, att.out_row_stride, att.out_head_stride = heads, rows, row_stride, head_stride
+        att.max_q_len = 1
+        assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == want
+        r.rows, r.k_row_stride, r.k_head_stride, r.v_row_stride, r.v_head_stride = rows, row_stride, head_stride, row_stride, head_stride
+        assert lib.mc_kv4_read(C.byref(cache), C.byref(r), None) == want
+    # more heads than a cache has: 2^31 - 2 of them, 2^33 apart
+    cache, r, att = host_args()
+    cache.batch, cache.kv_heads, att.max_q_len = 1, 1, 1
+    att.heads, att.q_rows, att.out_row_stride, att.out_head_stride = 2**30 - 1, 2**20, 64, 2**34 + 64
+    assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == sound
+    att.out_row_stride = 2**20
+    assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == L.MC_INVALID_INPUT
+    # strides whose bytes pass 64 bits
+    for stride in (2**62, 2**61 + 64, 2**40):
+        cache, r, att = host_args()
+        att.q_row_stride = stride
+        assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == L.MC_INVALID_INPUT
