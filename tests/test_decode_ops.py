@@ -8,6 +8,7 @@ the inputs that it was given, so no error adds up; tolerances as in each
 operator's own tests.
 """
 import ctypes as C
+import os
 
 import numpy as np
 import pytest
@@ -159,3 +160,57 @@ def test_host_memory_is_refused_wherever_it_is_given():
             ["logits", "temperature", "top_k", "top_p", "min_p", "uniform", "candidates", "tokens", "probs"])
     torch.cuda.synchronize()
     assert status_bits() == 0
+
+
+def documented_step():
+    """The Python lines of INTEGRATION.md's section on these operators."""
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    section = text[text.index("### Decode-step operators"):]
+    return section[section.index("```python\n") + len("```python\n"):].split("```")[0]
+
+
+@pytest.mark.parametrize("batch", [1, 3, 27, 28, 64])
+def test_the_documented_step(batch):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(batch)
+    rng = np.random.default_rng(batch)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    held = Cache(batch, 16, 16, 8, 64, fill=0xFF)
+    cs, lib, lens = held.struct(), L.load(), rng.integers(0, 255, batch)
+    past = [rnd(int(lens.sum()) + 1, 8, 64) for _ in range(2)]
+    before = rows_struct(*past, np.cumsum(lens) - lens, lens, np.zeros(batch), 255, L.MC_F32)
+    assert lib.mc_kv4_append(C.byref(cs), C.byref(before), torch.cuda.current_stream().cuda_stream) == L.MC_OK
+    src_len = rng.integers(1, 257, batch)
+    src_start = np.cumsum(src_len) - src_len
+    names = dict(
+        batch=batch, pages=held.pages, table=held.table_dev, n_pages=held.n_pages, k=rnd(batch, 8, 64), v=rnd(batch, 8, 64),
+        row=ints(np.arange(batch)), ones=ints(np.ones(batch)), length=ints(lens), length_plus_1=ints(lens + 1),
+        q=rnd(batch, 8, 64), out=torch.zeros(batch, 8, 64, device="cuda"), cq=rnd(batch, 8, 64),
+        co=torch.zeros(batch, 8, 64, device="cuda"), enc_k=rnd(int(src_len.sum()), 8, 64),
+        enc_v=rnd(int(src_len.sum()), 8, 64), src_start=ints(src_start), src_len=ints(src_len),
+        logits=rnd(batch, 32000) * 2, temperature=torch.full((batch,), 0.8, device="cuda"),
+        top_p=torch.full((batch,), 0.9, device="cuda"), uniform=torch.rand(batch, generator=g, device="cuda"),
+        tokens=torch.full((batch,), -7, dtype=torch.int32, device="cuda"), stream=torch.cuda.current_stream().cuda_stream)
+    exec(compile(documented_step(), "INTEGRATION.md", "exec"), names)
+    torch.cuda.synchronize()
+    assert status_bits() == 0
+    back = [torch.zeros(int(lens.sum()) + batch, 8, 64, device="cuda") for _ in range(2)]
+    total = lens + 1
+    at = np.cumsum(total) - total
+    read = rows_struct(*back, at, total, np.zeros(batch), 256, L.MC_F32)
+    assert lib.mc_kv4_read(C.byref(cs), C.byref(read), names["stream"]) == L.MC_OK
+    torch.cuda.synchronize()
+    q, out, cq, co, enc_k, enc_v = (f64(names[n]) for n in ("q", "out", "cq", "co", "enc_k", "enc_v"))
+    k, v = (f64(x) for x in back)
+    for i in range(batch):
+        ki, vi = k[at[i]:at[i] + total[i]], v[at[i]:at[i] + total[i]]
+        want, _ = kv_attend(q[i:i + 1], ki, vi, 0.125, lambda _: total[i])
+        tol = (2.0 ** -18 + 2 * score_error(q[i:i + 1], ki, 0.125)) * np.abs(vi).max()
+        np.testing.assert_allclose(out[i:i + 1], want, rtol=0, atol=tol)
+        src = slice(src_start[i], src_start[i] + src_len[i])
+        want, _ = cross_attend(cq[i:i + 1], enc_k[src], enc_v[src], 0.125, np.ones(src_len[i], bool))
+        dx = 2.0 ** -20 * 0.125 * np.abs(cq[i]).sum(-1).max() * np.abs(enc_k[src]).max()
+        np.testing.assert_allclose(co[i:i + 1], want, rtol=0, atol=(2.0 ** -18 + 2 * dx) * np.abs(enc_v[src]).max())
+        token, _ = sample_reference(f64(names["logits"])[i], float(np.float32(0.8)), 0, float(np.float32(0.9)), 0.0,
+                                    float(f64(names["uniform"])[i]))
+        assert int(names["tokens"][i]) == token
