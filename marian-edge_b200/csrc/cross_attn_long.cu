@@ -362,10 +362,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = 2; k < 32; k += 2) most[c] = max3(most[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       }
       const float high = max3(fmaxf(most[0], most[1]), most[2], most[3]);
-      if (__any_sync(kFull, __fmul_rn(__fsub_rn(high, top), factor) > kGrowth)) {
-        const float grown = fmaxf(top, high);
-        const float shrink = top == -INFINITY ? 0.0f : exp2_approx(__fmul_rn(__fsub_rn(top, grown), factor));
-        top = grown;
+      // a row goes by its own maximum alone, so that no other row of the warp
+      // (a NaN one, a batch's neighbour) has a part in its roundings
+      const bool grows = __fmul_rn(__fsub_rn(high, top), factor) > kGrowth;
+      if (__any_sync(kFull, grows)) {
+        const float shrink = !grows ? 1.0f : top == -INFINITY ? 0.0f : exp2_approx(__fmul_rn(__fsub_rn(top, high), factor));
+        if (grows) top = high;
         sum = __fmul_rn(sum, shrink);
         if (j > 0) {
 #pragma unroll

@@ -562,3 +562,24 @@ def test_overlaps_of_wide_strides_are_refused():
     a.out_head_stride = 2**18
     sound = L.MC_INVALID_INPUT if torch.cuda.is_available() else L.MC_CUDA   # past the checks; there is no such memory
     assert L.load().mc_cross_attention(C.byref(a), None) == sound
+
+
+# ---- the long tiles' edges: 128 rows or more, two key tiles or more, 16 bits, no mask ----
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("b,q_len,n,d", [(1, 128, 200, 64), (2, 300, 700, 128), (200, 130, 300, 64), (1, 260, 5000, 48)])
+def test_long_tiles_keep_a_nan_query_to_its_row(dtype, b, q_len, n, d):
+    rng = np.random.default_rng(n)
+    q, k, v = typed(rng, (b * q_len, 2, d), dtype, 4.0), typed(rng, (n, 2, d), dtype), typed(rng, (n, 2, d), dtype)
+    k *= torch.linspace(0.2, 2.0, n).to(k.dtype)[:, None, None]        # maxima grow on the way: rows are rescaled
+    args = (np.arange(b) * q_len, [q_len] * b, [0] * b, [n] * b, dtype, d ** -0.5)
+    good, gl, _ = run(q.cuda(), k.cuda(), v.cuda(), *args)
+    spoilt = [(2, 1), (q_len - 1, 0), ((b - 1) * q_len + 65, 1), (b * q_len - 1, 0)]
+    same = torch.ones(b * q_len, 2, dtype=torch.bool, device="cuda")
+    for i, (row, head) in enumerate(spoilt):
+        q[row, head, i * 7 % d] = float("nan")
+        same[row, head] = False
+    out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), *args)
+    assert torch.equal(out[same], good[same]) and torch.equal(lse[same], gl[same])
+    assert bool(out[~same].isnan().all()) and bool(lse[~same].isnan().all()) and bool(good.isfinite().all())
