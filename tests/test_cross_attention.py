@@ -583,3 +583,93 @@ def test_long_tiles_keep_a_nan_query_to_its_row(dtype, b, q_len, n, d):
     out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), *args)
     assert torch.equal(out[same], good[same]) and torch.equal(lse[same], gl[same])
     assert bool(out[~same].isnan().all()) and bool(lse[~same].isnan().all()) and bool(good.isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_long_tiles_on_infinities(dtype):
+    # a key whose score is -inf for every query weighs nothing; an infinite value makes its channel infinite
+    rng, n, q_len = np.random.default_rng(3), 300, 150
+    q, k, v = (typed(rng, (m, 2, 64), dtype) for m in (q_len, n, n))
+    q = q.abs() + 0.1
+    k[140, 0, 3], v[200, 1, 5], v[7, 1, 6] = -float("inf"), float("inf"), -float("inf")
+    out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), [0], [q_len], [0], [n], dtype, 0.125)
+    rest = np.ones(n, bool)
+    rest[140] = False
+    qd, kd, vd, od = (f64(x) for x in (q, k, v, out))
+    want, wl = attend(qd, np.where(np.isfinite(kd), kd, 0.0), np.where(np.isfinite(vd), vd, 0.0), 0.125, rest)
+    dx = 2.0 ** -20 * 0.125 * np.abs(qd).sum(-1).max() * np.abs(kd[np.isfinite(kd)]).max()
+    tol = (torch.finfo(q.dtype).eps + 2 * dx) * np.abs(vd[np.isfinite(vd)]).max()
+    np.testing.assert_allclose(od[:, 0], want[:, 0], rtol=0, atol=tol)
+    np.testing.assert_allclose(f64(lse)[:, 0], wl[:, 0], rtol=2.0 ** -20, atol=2.0 ** -19 + dx)
+    assert (od[:, 1, 5] == np.inf).all() and (od[:, 1, 6] == -np.inf).all() and np.isfinite(od[:, 1, 7:]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,size", [("bf16", 250.0), ("f16", 250.0), ("bf16", 250000.0)])
+def test_long_tiles_on_scores_far_from_zero(dtype, size):
+    # every score of a half near +-size * 16: equal scores share the weight, and the half below has none
+    rng, n = np.random.default_rng(9), 300
+    for high in (slice(0, 150), slice(150, 300), slice(100, 103)):
+        q = torch.full((140, 1, 64), 2.0).to(DTYPES[dtype][0])
+        k = torch.full((n, 1, 64), -size)
+        k[high] = size
+        k, v = k.to(q.dtype), typed(rng, (n, 1, 64), dtype)
+        out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), [0], [140], [0], [n], dtype, 0.125)
+        want, one = f64(v)[high].mean(0), f64(k)[high][0, 0, 0]
+        np.testing.assert_allclose(f64(out), np.broadcast_to(want, out.shape),
+                                   atol=torch.finfo(q.dtype).eps * np.abs(f64(v)).max())
+        np.testing.assert_allclose(f64(lse), 16.0 * one + np.log(high.stop - high.start), rtol=2.0 ** -20)
+        q[:] = -2.0     # now the other half is above
+        out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), [0], [140], [0], [n], dtype, 0.125)
+        rest = np.ones(n, bool)
+        rest[high] = False
+        np.testing.assert_allclose(f64(out), np.broadcast_to(f64(v)[rest].mean(0), out.shape),
+                                   atol=torch.finfo(q.dtype).eps * np.abs(f64(v)).max())
+
+
+@gpu
+def test_long_tiles_past_4_gib():
+    # keys and values whose byte offsets pass 2^32, the sequence's the last rows; several key tiles and a
+    # rest, and heads at 2^31 bytes too
+    rng, rows, hk, d, n = np.random.default_rng(5), 300_000, 64, 128, 333
+    k = torch.empty(rows, hk, d, dtype=torch.bfloat16, device="cuda")
+    q, kv = typed(rng, (140, hk, d), "bf16"), typed(rng, (n, hk, d), "bf16")
+    k[rows - n:] = kv.cuda()
+    out, lse, _ = run(q.cuda(), k, k, [0], [140], [rows - n], [n], "bf16", d ** -0.5)
+    compare(q, kv, kv, out, lse, [0], [140], [0], [n], "bf16", d ** -0.5)
+    by_head = k.view(hk, rows, d)      # head-major: a head's rows are 77 MB apart from the next one's
+    by_head[:, rows - n:] = kv.cuda().transpose(0, 1)
+    turned = by_head.transpose(0, 1)
+    out, lse, _ = run(q.cuda(), turned, turned, [0], [140], [rows - n], [n], "bf16", d ** -0.5)
+    compare(q, kv, kv, out, lse, [0], [140], [0], [n], "bf16", d ** -0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_long_tiles_of_several_queries_of_one_source(dtype):
+    rng = np.random.default_rng(1)
+    q, k, v = typed(rng, (600, 4, 64), dtype), typed(rng, (500, 2, 64), dtype), typed(rng, (500, 2, 64), dtype)
+    q_start, q_len, k_start, k_len = [0, 300, 430], [290, 130, 170], [3, 3, 110], [390, 390, 333]
+    out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), q_start, q_len, k_start, k_len, dtype, 0.125)
+    compare(q, k, v, out, lse, q_start, q_len, k_start, k_len, dtype, 0.125)
+
+
+@gpu
+@pytest.mark.parametrize("field,value", [("q_start", -1), ("q_start", 1 << 20), ("q_len", -1), ("q_len", 301), ("k_start", -1),
+                                         ("k_start", 3000), ("k_len", 1101), ("k_len", -5), ("k_start", 2147483647)])
+@pytest.mark.parametrize("b,heads", [(3, 2), (80, 4)])     # cut into ranges; several waves, the last one cut
+def test_long_tiles_leave_bad_lengths_out(field, value, b, heads):
+    rng = np.random.default_rng(4)
+    q = typed(rng, (300 * b, heads, 32), "bf16").cuda()
+    k, v = (typed(rng, (3000, heads, 32), "bf16").cuda() for _ in range(2))
+    given = {"q_start": np.arange(b) * 300, "q_len": np.full(b, 300), "k_start": np.arange(b) * 7, "k_len": np.full(b, 1100)}
+    good, gl, need = run(q, k, v, *given.values(), "bf16", 0.2, max_q=300, max_k=1100)
+    assert status_bits() == 0 and need > 0
+    given[field][b - 2] = value
+    out, lse, _ = run(q, k, v, *given.values(), "bf16", 0.2, max_q=300, max_k=1100)
+    assert status_bits() == 4
+    left = torch.zeros(300 * b, dtype=torch.bool, device="cuda")
+    left[(b - 2) * 300:(b - 1) * 300] = True
+    assert torch.equal(out[~left], good[~left]) and torch.equal(lse[~left], gl[~left])
+    assert bool((out[left] == 7).all()) and bool((lse[left] == 7).all())
