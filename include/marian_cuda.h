@@ -409,7 +409,7 @@ typedef struct {
     int32_t heads;               /* a multiple of the cache's kv_heads */
     int32_t max_q_len, max_kv_len;  /* no q_len[b] / kv_len[b] is above them; max_kv_len <= 2^31 - 256 */
     int32_t causal;
-    float scale;                 /* finite, commonly 1 / sqrt(head_dim) */
+    float scale;                 /* finite, below 2.35e38; commonly 1 / sqrt(head_dim) */
 } mc_kv4_attention_args;
 
 /* Workspace bytes for a call with these sizes (pointers are not looked at);
@@ -447,7 +447,7 @@ typedef struct {
     int32_t batch, heads, kv_heads;  /* heads a multiple of kv_heads */
     int32_t head_dim;            /* a multiple of 16, 16..128 */
     int32_t max_q_len, max_k_len;  /* no q_len[b] / k_len[b] is above them; max_k_len <= 2^31 - 256 */
-    float scale;                 /* finite, commonly 1 / sqrt(head_dim) */
+    float scale;                 /* finite, below 2.35e38; commonly 1 / sqrt(head_dim) */
 } mc_cross_attention_args;
 
 /* Workspace bytes for a call with these sizes (pointers are not looked at);

@@ -709,7 +709,7 @@ extern "C" uint64_t mc_cross_attention_workspace(const mc_cross_attention_args* 
 }
 
 extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* stream) {
-  if (!mc::cross_sizes_ok(a) || !isfinite(a->scale) || a->q_rows < 0 || a->q_rows > INT32_MAX || a->k_rows < 0 ||
+  if (!mc::cross_sizes_ok(a) || !mc::scale_ok(a->scale) || a->q_rows < 0 || a->q_rows > INT32_MAX || a->k_rows < 0 ||
       a->k_rows > INT32_MAX)
     return MC_INVALID_INPUT;
   if (a->batch == 0 || a->max_q_len == 0) return MC_OK;

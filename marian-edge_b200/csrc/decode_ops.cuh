@@ -174,6 +174,9 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 inline int dtype_bytes(int32_t dtype) { return dtype == MC_F32 ? 4 : dtype == MC_F16 || dtype == MC_BF16 ? 2 : 0; }
 
+// The scale of scores in powers of two has to be a number.
+inline bool scale_ok(float scale) { return isfinite(scale * kLog2e); }
+
 // Memory of another device or pageable host memory is refused, for every
 // pointer that is given (70 ns each); memory that CUDA says nothing about
 // cannot be read by a kernel either.

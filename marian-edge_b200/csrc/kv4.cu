@@ -1102,7 +1102,7 @@ extern "C" uint64_t mc_kv4_attention_workspace(const mc_kv4_cache* cache, const 
 
 extern "C" mc_status mc_kv4_attention(const mc_kv4_cache* c, const mc_kv4_attention_args* a, void* stream) {
   mc::Kv4Plan plan;
-  if (!mc::kv4_plan(c, a, &plan) || !isfinite(a->scale) || a->q_rows < 0 || a->q_rows > INT32_MAX)
+  if (!mc::kv4_plan(c, a, &plan) || !mc::scale_ok(a->scale) || a->q_rows < 0 || a->q_rows > INT32_MAX)
     return MC_INVALID_INPUT;
   if (plan.units == 0) return MC_OK;
   const int bytes = mc::dtype_bytes(a->dtype);

@@ -673,3 +673,12 @@ def test_long_tiles_leave_bad_lengths_out(field, value, b, heads):
     left[(b - 2) * 300:(b - 1) * 300] = True
     assert torch.equal(out[~left], good[~left]) and torch.equal(lse[~left], gl[~left])
     assert bool((out[left] == 7).all()) and bool((lse[left] == 7).all())
+
+
+def test_scales_past_the_largest_power_of_two_are_refused():
+    # scores are taken in powers of two: scale * log2(e) has to be a number
+    for scale, sound in ((2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False)):
+        a = host_args()
+        a.scale = scale
+        got = L.load().mc_cross_attention(C.byref(a), None)
+        assert got == (L.MC_CUDA if sound and not torch.cuda.is_available() else L.MC_INVALID_INPUT)

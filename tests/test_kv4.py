@@ -827,3 +827,12 @@ def test_overlaps_of_wide_strides_are_refused():
         cache, r, att = host_args()
         att.q_row_stride = stride
         assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == L.MC_INVALID_INPUT
+
+
+def test_scales_past_the_largest_power_of_two_are_refused():
+    # scores are taken in powers of two: scale * log2(e) has to be a number
+    for scale, sound in ((2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False)):
+        cache, _, att = host_args()
+        att.scale = scale
+        got = L.load().mc_kv4_attention(C.byref(cache), C.byref(att), None)
+        assert got == (L.MC_CUDA if sound and not torch.cuda.is_available() else L.MC_INVALID_INPUT)
