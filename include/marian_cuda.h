@@ -324,8 +324,9 @@ mc_status mc_op_status(uint32_t *status_bits);
  *
  * Every pointer in the structs below is a device pointer of the current
  * device (managed memory, or mapped host memory at its own address, will do;
- * anything else is refused), arrays are dense unless they come with
- * strides, and strides count elements.  The struct itself is read during the
+ * anything else is refused; a tensor of no rows, or a cache of no pages, may
+ * be null), arrays are dense unless they come with strides, and strides
+ * count elements.  The struct itself is read during the
  * call.  The calls are asynchronous on `stream` (a cudaStream_t of the current
  * device, 0 = default), allocate nothing and can be captured in a CUDA graph
  * (the first call on a device sets up the status word: make one before any

@@ -716,12 +716,12 @@ extern "C" mc_status mc_cross_attention(const mc_cross_attention_args* a, void* 
   const int bytes = mc::dtype_bytes(a->dtype);
   if (!a->q_start || !a->q_len || !a->k_start || !a->k_len || !mc::aligned4(a->q_start) || !mc::aligned4(a->q_len) ||
       !mc::aligned4(a->k_start) || !mc::aligned4(a->k_len) || !mc::aligned4(a->lse) ||
-      !mc::strides_ok(a->q, a->q_row_stride, a->q_head_stride, bytes) ||
-      !mc::strides_ok(a->k, a->k_row_stride, a->k_head_stride, bytes) ||
-      !mc::strides_ok(a->v, a->v_row_stride, a->v_head_stride, bytes) ||
-      !mc::strides_ok(a->out, a->out_row_stride, a->out_head_stride, bytes) ||
-      !mc::strides_apart(a->q_rows, a->heads, a->head_dim, a->out_row_stride, a->out_head_stride) || a->out == a->q ||
-      a->out == a->k || a->out == a->v)
+      !mc::strides_ok(a->q, a->q_rows, a->q_row_stride, a->q_head_stride, bytes) ||
+      !mc::strides_ok(a->k, a->k_rows, a->k_row_stride, a->k_head_stride, bytes) ||
+      !mc::strides_ok(a->v, a->k_rows, a->v_row_stride, a->v_head_stride, bytes) ||
+      !mc::strides_ok(a->out, a->q_rows, a->out_row_stride, a->out_head_stride, bytes) ||
+      !mc::strides_apart(a->q_rows, a->heads, a->head_dim, a->out_row_stride, a->out_head_stride) ||
+      (a->out && (a->out == a->q || a->out == a->k || a->out == a->v)))
     return MC_INVALID_INPUT;
   const uint64_t need = mc_cross_attention_workspace(a);
   if (need > 0 && (!a->workspace || !mc::aligned16(a->workspace) || a->workspace_bytes < need)) return MC_INVALID_INPUT;

@@ -205,10 +205,11 @@ inline mc_status launched(cudaError_t e) {
   return MC_CUDA;
 }
 
-// Rows of head_dim values whose strides keep every 16-byte load aligned.
+// Rows of head_dim values whose strides keep every 16-byte load aligned.  No
+// rows need no address: an empty tensor's is often null.
 constexpr int64_t kOpMaxStride = int64_t(1) << 40;
-inline bool strides_ok(const void* base, int64_t row_stride, int64_t head_stride, int bytes) {
-  return base && aligned16(base) && row_stride >= 0 && head_stride >= 0 && row_stride < kOpMaxStride &&
+inline bool strides_ok(const void* base, int64_t rows, int64_t row_stride, int64_t head_stride, int bytes) {
+  return (base || rows == 0) && aligned16(base) && row_stride >= 0 && head_stride >= 0 && row_stride < kOpMaxStride &&
          head_stride < kOpMaxStride && (row_stride * bytes) % 16 == 0 && (head_stride * bytes) % 16 == 0;
 }
 

@@ -1049,13 +1049,13 @@ mc_status kv4_rows(const mc_kv4_cache* c, const mc_kv4_rows* a, void* stream) {
   if (!kv4_cache_ok(c) || !a || bytes == 0 || a->rows < 0 || a->rows > INT32_MAX || a->max_count < 0) return MC_INVALID_INPUT;
   if (c->batch == 0 || a->max_count == 0) return MC_OK;
   const long long chunks = (a->max_count + (long long)kRowTokens - 1) / kRowTokens, grid = chunks * c->batch;
-  if (grid > INT32_MAX || !c->pages || !aligned16(c->pages) || !c->page_table || !aligned4(c->page_table) ||
+  if (grid > INT32_MAX || (!c->pages && c->n_pages > 0) || !aligned16(c->pages) || !c->page_table || !aligned4(c->page_table) ||
       !a->start || !a->count || !a->first || !aligned4(a->start) || !aligned4(a->count) || !aligned4(a->first) ||
-      !strides_ok(a->k, a->k_row_stride, a->k_head_stride, bytes) ||
-      !strides_ok(a->v, a->v_row_stride, a->v_head_stride, bytes))
+      !strides_ok(a->k, a->rows, a->k_row_stride, a->k_head_stride, bytes) ||
+      !strides_ok(a->v, a->rows, a->v_row_stride, a->v_head_stride, bytes))
     return MC_INVALID_INPUT;
   if (READ && (!strides_apart(a->rows, c->kv_heads, c->head_dim, a->k_row_stride, a->k_head_stride) ||
-               !strides_apart(a->rows, c->kv_heads, c->head_dim, a->v_row_stride, a->v_head_stride) || a->k == a->v))
+               !strides_apart(a->rows, c->kv_heads, c->head_dim, a->v_row_stride, a->v_head_stride) || (a->k && a->k == a->v)))
     return MC_INVALID_INPUT;
   const mc_status where = on_current_device({c->pages, c->page_table, a->k, a->v, a->start, a->count, a->first});
   if (where != MC_OK) return where;
@@ -1106,12 +1106,13 @@ extern "C" mc_status mc_kv4_attention(const mc_kv4_cache* c, const mc_kv4_attent
     return MC_INVALID_INPUT;
   if (plan.units == 0) return MC_OK;
   const int bytes = mc::dtype_bytes(a->dtype);
-  if (a->max_kv_len > (int64_t)c->pages_per_seq * c->page_tokens || !c->pages || !mc::aligned16(c->pages) ||
+  if (a->max_kv_len > (int64_t)c->pages_per_seq * c->page_tokens || (!c->pages && c->n_pages > 0) || !mc::aligned16(c->pages) ||
       !c->page_table || !mc::aligned4(c->page_table) || !a->q_start || !a->q_len || !a->kv_len ||
       !mc::aligned4(a->q_start) || !mc::aligned4(a->q_len) || !mc::aligned4(a->kv_len) || !mc::aligned4(a->lse) ||
-      !mc::strides_ok(a->q, a->q_row_stride, a->q_head_stride, bytes) ||
-      !mc::strides_ok(a->out, a->out_row_stride, a->out_head_stride, bytes) ||
-      !mc::strides_apart(a->q_rows, a->heads, c->head_dim, a->out_row_stride, a->out_head_stride) || a->q == a->out)
+      !mc::strides_ok(a->q, a->q_rows, a->q_row_stride, a->q_head_stride, bytes) ||
+      !mc::strides_ok(a->out, a->q_rows, a->out_row_stride, a->out_head_stride, bytes) ||
+      !mc::strides_apart(a->q_rows, a->heads, c->head_dim, a->out_row_stride, a->out_head_stride) ||
+      (a->out && a->q == a->out))
     return MC_INVALID_INPUT;
   if (plan.bytes > 0 && (!a->workspace || !mc::aligned16(a->workspace) || a->workspace_bytes < plan.bytes))
     return MC_INVALID_INPUT;

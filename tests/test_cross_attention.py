@@ -682,3 +682,30 @@ def test_scales_past_the_largest_power_of_two_are_refused():
         a.scale = scale
         got = L.load().mc_cross_attention(C.byref(a), None)
         assert got == (L.MC_CUDA if sound and not torch.cuda.is_available() else L.MC_INVALID_INPUT)
+
+
+def test_tensors_of_no_rows_may_be_null():
+    lib = L.load()
+    a = host_args()
+    a.q, a.out, a.q_rows, a.k, a.v, a.k_rows = None, None, 0, None, None, 0
+    sound = L.MC_INVALID_INPUT if torch.cuda.is_available() else L.MC_CUDA   # past the checks; there is no such memory
+    assert lib.mc_cross_attention(C.byref(a), None) == sound
+    for field in ("q_rows", "k_rows"):
+        setattr(a, field, 1)
+        assert lib.mc_cross_attention(C.byref(a), None) == L.MC_INVALID_INPUT
+        setattr(a, field, 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-30, 1.5])
+@pytest.mark.parametrize("q_len", [1, 150])
+def test_scales_of_any_sign(dtype, scale, q_len):
+    rng = np.random.default_rng(q_len)
+    q, k, v = (typed(rng, (n, 2, 64), dtype) for n in (q_len, 260, 260))
+    out, lse, _ = run(q.cuda(), k.cuda(), v.cuda(), [0], [q_len], [0], [260], dtype, scale)
+    want, wl = attend(f64(q), f64(k), f64(v), float(np.float32(scale)), np.ones(260, bool))
+    dx = 2.0 ** -20 * abs(scale) * np.abs(f64(q)).sum(-1).max() * np.abs(f64(k)).max()
+    tol = (2.0 ** -18 if dtype == "f32" else torch.finfo(q.dtype).eps) + 2 * dx
+    np.testing.assert_allclose(f64(out), want, rtol=0, atol=tol * np.abs(f64(v)).max())
+    np.testing.assert_allclose(f64(lse), wl, rtol=2.0 ** -20, atol=2.0 ** -19 + dx)

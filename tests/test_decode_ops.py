@@ -214,3 +214,52 @@ def test_the_documented_step(batch):
         token, _ = sample_reference(f64(names["logits"])[i], float(np.float32(0.8)), 0, float(np.float32(0.9)), 0.0,
                                     float(f64(names["uniform"])[i]))
         assert int(names["tokens"][i]) == token
+
+
+@pytest.mark.parametrize("code", [L.MC_F32, L.MC_BF16])
+@pytest.mark.parametrize("q_len", [1, 200])
+def test_tensors_of_no_rows_may_be_null(code, q_len):
+    # no keys at all, no queries, no new rows, no pages: nothing is read, and a length that says otherwise
+    # is reported
+    lib, stream = L.load(), torch.cuda.current_stream().cuda_stream
+    dtype = torch.float32 if code == L.MC_F32 else torch.bfloat16
+    zero, one, full = ints([0, 0]), ints([1, 1]), ints([q_len, 0])
+    q, out, lse = torch.ones(q_len, 2, 64, dtype=dtype, device="cuda"), torch.full((q_len, 2, 64), 7.0, dtype=dtype, device="cuda"), torch.zeros(q_len, 2, device="cuda")
+    strides = dict(q_row_stride=128, q_head_stride=64, out_row_stride=128, out_head_stride=64)
+    rows = dict(q=q.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(), q_start=zero.data_ptr(), q_len=full.data_ptr())
+    room = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    kv = dict(k_row_stride=128, k_head_stride=64, v_row_stride=128, v_head_stride=64)
+    cross = L.CrossAttentionArgs(**rows, **strides, **kv, k_start=zero.data_ptr(), k_len=zero.data_ptr(), q_rows=q_len, k_rows=0,
+                                 workspace=room.data_ptr(), workspace_bytes=1 << 24, dtype=code, batch=2, heads=2,
+                                 kv_heads=2, head_dim=64, max_q_len=q_len, max_k_len=300, scale=0.125)
+    assert lib.mc_cross_attention(C.byref(cross), stream) == L.MC_OK and status_bits() == 0
+    assert bool((out == 0).all()) and bool(lse.isneginf().all())
+    cross.k_len = one.data_ptr()      # both sequences say that they have a key
+    out.fill_(7.0)
+    assert lib.mc_cross_attention(C.byref(cross), stream) == L.MC_OK and status_bits() == 4
+    assert bool((out == 7).all())
+    table = ints([0, 0])
+    cache = L.Kv4Cache(page_table=table.data_ptr(), n_pages=0, page_tokens=16, kv_heads=2, head_dim=64, batch=2, pages_per_seq=1)
+    att = L.Kv4AttentionArgs(**rows, **strides, kv_len=zero.data_ptr(), q_rows=q_len, workspace=room.data_ptr(),
+                             workspace_bytes=1 << 24, dtype=code, heads=2, max_q_len=q_len, max_kv_len=16, scale=0.125)
+    assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), stream) == L.MC_OK and status_bits() == 0
+    assert bool((out == 0).all()) and bool(lse.isneginf().all())
+    att.kv_len = one.data_ptr()       # a page that is not there
+    assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), stream) == L.MC_OK and status_bits() == 4
+    new = L.Kv4Rows(start=zero.data_ptr(), count=zero.data_ptr(), first=zero.data_ptr(), rows=0, **kv, dtype=code, max_count=3)
+    for fn in (lib.mc_kv4_append, lib.mc_kv4_read):
+        new.count = zero.data_ptr()
+        assert fn(C.byref(cache), C.byref(new), stream) == L.MC_OK and status_bits() == 0
+        new.count = one.data_ptr()
+        assert fn(C.byref(cache), C.byref(new), stream) == L.MC_OK and status_bits() == 4
+    att.q_rows, att.q, att.out, att.lse, att.kv_len = 0, None, None, None, zero.data_ptr()
+    cross.q_rows, cross.q, cross.out, cross.lse, cross.k_len = 0, None, None, None, zero.data_ptr()
+    for lens, bits in ((zero, 0), (one, 4)):
+        att.q_len = cross.q_len = lens.data_ptr()
+        assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), stream) == L.MC_OK and status_bits() == bits
+        assert lib.mc_cross_attention(C.byref(cross), stream) == L.MC_OK and status_bits() == bits
+    for struct, field in ((cross, "k_rows"), (cross, "q_rows"), (att, "q_rows")):
+        setattr(struct, field, 1)
+        assert (lib.mc_cross_attention(C.byref(struct), stream) if struct is cross else
+                lib.mc_kv4_attention(C.byref(cache), C.byref(struct), stream)) == L.MC_INVALID_INPUT
+        setattr(struct, field, 0)

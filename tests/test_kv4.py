@@ -836,3 +836,36 @@ def test_scales_past_the_largest_power_of_two_are_refused():
         att.scale = scale
         got = L.load().mc_kv4_attention(C.byref(cache), C.byref(att), None)
         assert got == (L.MC_CUDA if sound and not torch.cuda.is_available() else L.MC_INVALID_INPUT)
+
+
+def test_tensors_of_no_rows_may_be_null():
+    lib = L.load()
+    sound = L.MC_INVALID_INPUT if torch.cuda.is_available() else L.MC_CUDA   # past the checks; there is no such memory
+    cache, rows, att = host_args()
+    rows.k, rows.v, rows.rows = None, None, 0
+    att.q, att.out, att.q_rows = None, None, 0
+    cache.pages, cache.n_pages = None, 0
+    assert lib.mc_kv4_append(C.byref(cache), C.byref(rows), None) == sound
+    assert lib.mc_kv4_read(C.byref(cache), C.byref(rows), None) == sound
+    assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == sound
+    rows.rows = att.q_rows = 1
+    assert lib.mc_kv4_read(C.byref(cache), C.byref(rows), None) == L.MC_INVALID_INPUT
+    assert lib.mc_kv4_attention(C.byref(cache), C.byref(att), None) == L.MC_INVALID_INPUT
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-30, 1.5])
+def test_scales_of_any_sign(dtype, scale):
+    rng = np.random.default_rng(31)
+    cache = Cache(2, 9, 16, 2, 64)
+    ks, vs = filled(rng, cache, [140, 77])
+    q = typed(rng, (8, 4, 64), dtype)
+    out, lse, _ = attention(cache, q.cuda(), [0, 4], [4, 4], [140, 77], scale, 1, dtype)
+    for i, n in enumerate((140, 77)):
+        at = slice(4 * i, 4 * i + 4)
+        want, wl = attend(f64(q)[at], ks[i], vs[i], float(np.float32(scale)), lambda j: n - (3 - j))
+        dx = score_error(f64(q)[at], ks[i], abs(scale))
+        tol = (2.0 ** -18 if dtype == "f32" else torch.finfo(q.dtype).eps / 2 + 2.0 ** -11) + 2 * dx
+        np.testing.assert_allclose(f64(out)[at], want, rtol=0, atol=tol * np.abs(vs[i]).max())
+        np.testing.assert_allclose(f64(lse)[at], wl, rtol=2.0 ** -20, atol=2.0 ** -19 + dx)
