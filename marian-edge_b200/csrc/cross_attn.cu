@@ -12,7 +12,6 @@ namespace mc {
 namespace {
 
 constexpr uint32_t kFull = 0xFFFFFFFFu;
-constexpr int kSms = 148;
 
 // ---- small tiles: mma.sync ------------------------------------------------------------
 // Four warps: WR of them side by side over 16 rows each, the other 4 / WR

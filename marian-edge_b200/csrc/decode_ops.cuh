@@ -19,6 +19,7 @@ namespace mc {
 // nullptr when there is none to be had.
 uint32_t* op_status_word();
 
+constexpr int kSms = 148;
 constexpr int kOpMaxHeadDim = 128;
 constexpr int kOpMaxKeys = INT32_MAX - 255;  // of a sequence: positions a tile further on still are an int
 constexpr float kLog2e = 1.4426950408889634f;

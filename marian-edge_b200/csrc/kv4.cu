@@ -956,8 +956,6 @@ struct Kv4Plan {
   uint64_t slots, bytes;
 };
 
-constexpr int kSms = 148;
-
 bool kv4_shape_ok(int32_t page_tokens, int32_t kv_heads, int32_t head_dim) {
   return (page_tokens == 8 || page_tokens == 16 || page_tokens == 32) && kv_heads >= 1 && kv_heads <= 65536 &&
          head_dim >= 16 && head_dim <= kOpMaxHeadDim && head_dim % 16 == 0;

@@ -165,7 +165,7 @@ struct Weigher {
 // What the CTAs of a row tell one another; two of each, used in turn, so
 // that one cluster barrier per exchange is enough.
 struct Exchange {
-  unsigned long long value[2][3];
+  unsigned long long value[2][2];
 };
 
 struct Shared {
@@ -173,7 +173,7 @@ struct Shared {
     unsigned long long hist[2][kBins];  // the general way
     unsigned long long list[kList];     // candidates: key, then ~id
   };
-  uint32_t counts[kCoarse];      // tokens per bin, of the sample, the list or the slice
+  uint32_t counts[kCoarse];      // tokens of this slice per bin; in a long list's draw, weights per range of ids
   uint32_t starts[kCoarse + 1];  // of the whole row, up to each bin
   uint32_t filled[kCoarse];      // candidates of each bin that have arrived
   uint32_t listed;               // tokens of a border's bin
@@ -187,14 +187,6 @@ template <typename V>
 __device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-  return v;
-}
-__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long w = __shfl_xor_sync(kFull, v, o);
-    v = w > v ? w : v;
-  }
   return v;
 }
 template <typename V>
@@ -265,18 +257,14 @@ struct Row {
   }
 
   // ---- reductions over the row ----
-  template <bool MAX>
-  __device__ __forceinline__ unsigned long long block(unsigned long long v) {
-    v = MAX ? warp_max(v) : warp_sum(v);
+  __device__ __forceinline__ unsigned long long block_sum(unsigned long long v) {
+    v = warp_sum(v);
     __syncthreads();
     if (lane == 0) sh.warp_value[warp] = v;
     __syncthreads();
     v = sh.warp_value[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) {
-      const unsigned long long o = sh.warp_value[w];
-      v = MAX ? (o > v ? o : v) : v + o;
-    }
+    for (int w = 1; w < kWarps; ++w) v += sh.warp_value[w];
     return v;
   }
   // The largest of two values over the block, in one exchange.
@@ -294,12 +282,11 @@ struct Row {
     }
   }
   // Publishes this CTA's values; afterwards peer(r, i) reads those of CTA r.
-  __device__ __forceinline__ void publish(unsigned long long a, unsigned long long b, unsigned long long c) {
+  __device__ __forceinline__ void publish(unsigned long long a, unsigned long long b = 0) {
     turn ^= 1;
     if (tid == 0) {
       sh.out.value[turn][0] = a;
       sh.out.value[turn][1] = b;
-      sh.out.value[turn][2] = c;
     }
     cluster.sync();
   }
@@ -455,7 +442,7 @@ struct Row {
       __syncthreads();
       found = sh.found[0];
     }
-    publish(found, 0, 0);
+    publish(found);
     found = peer(0, 0);
     if (!found) return false;
     cut->key = (uint32_t)(found >> 32);
@@ -475,31 +462,28 @@ struct Row {
     return warp_sum(s);
   }
   // The id for a target, from the sums of f before and after each warp's
-  // segment (one warp's `after` is the next one's `before`, to the bit); -1 in the CTAs that do not hold it.  The warp that does
-  // shares its segment out over the block, and then each warp's part is short.
-  // Sums in double may come out a little different there: a target past the
-  // last part's sum is the last id with a weight.
-  template <typename V, typename F>
-  __device__ int locate(F f, V before, V after, V target) {
-    auto bits = [](V v) { unsigned long long b; memcpy(&b, &v, 8); return b; };
-    auto from_bits = [](unsigned long long b) { V v; memcpy(&v, &b, 8); return v; };
+  // segment (one warp's `after` is the next one's `before`); -1 in the CTAs that
+  // do not hold it.  The warp that does shares its segment out over the block,
+  // until each warp's part is short.
+  template <typename F>
+  __device__ int locate(F f, unsigned long long before, unsigned long long after, unsigned long long target) {
     __syncthreads();
     if (tid == 0) sh.found[0] = kWarps;
     __syncthreads();
     if (lane == 0 && before <= target && target < after) {
       sh.found[0] = warp;
-      sh.found[1] = bits(before);
+      sh.found[1] = before;
     }
     __syncthreads();
     const int owner = (int)sh.found[0];
     if (owner == kWarps) return -1;  // the whole block
-    before = from_bits(sh.found[1]);
+    before = sh.found[1];
     int lo = owner * p.segment, hi = min(n, lo + p.segment);
     constexpr int kFew = 16;  // loads that one warp has in flight at the end
     while (hi - lo > 32 * kFew) {
       const int part = ((hi - lo) / 32 + kWarps - 1) / kWarps * 32 + 32;
       const int begin = min(hi, lo + warp * part), stop = min(hi, begin + part);
-      V sum = 0;
+      unsigned long long sum = 0;
 #pragma unroll 4
       for (int i = begin + lane; i < stop; i += 32) {
         const float v = at(i);
@@ -507,14 +491,14 @@ struct Row {
       }
       sum = warp_sum(sum);
       __syncthreads();
-      if (lane == 0) sh.warp_value[warp] = bits(sum);
+      if (lane == 0) sh.warp_value[warp] = sum;
       __syncthreads();
-      V run = before, start = before;
+      unsigned long long run = before, start = before;
       int mine = 0;  // the first part whose sum passes the target, or the last with any
       bool hit = false;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const V s = from_bits(sh.warp_value[w]);
+        const unsigned long long s = sh.warp_value[w];
         if (s > 0 && !hit) {
           mine = w;
           start = run;
@@ -536,8 +520,8 @@ struct Row {
       for (int k = 0; k < kFew; ++k) {
         const int i = lo + 32 * k;
         if (hit || i >= hi) continue;
-        const V w = i + lane < hi ? f(v[k], key_of(v[k]), base + i + lane) : V(0);
-        const V inc = before + warp_prefix(w, lane);
+        const unsigned long long w = i + lane < hi ? f(v[k], key_of(v[k]), base + i + lane) : 0ull;
+        const unsigned long long inc = before + warp_prefix(w, lane);
         const uint32_t past = __ballot_sync(kFull, w > 0 && inc > target), some = __ballot_sync(kFull, w > 0);
         if (some) id = base + i + 31 - __clz(some);
         if (past) {
@@ -562,7 +546,7 @@ struct Row {
       if (w < warp) before += sh.warp_value[w];
       own += sh.warp_value[w];
     }
-    publish(own, 0, 0);
+    publish(own);
     *total = 0;
     for (int r = 0; r < ranks; ++r) {
       const unsigned long long o = peer(r, 0);
@@ -577,8 +561,8 @@ struct Row {
     const unsigned long long sum = segment_sum(one);
     unsigned long long total;
     const unsigned long long before = prefix(sum, &total);
-    const int id = locate<unsigned long long>(one, before, before + sum, count - 1);
-    publish((unsigned long long)(id + 1), 0, 0);
+    const int id = locate(one, before, before + sum, count - 1);
+    publish((unsigned long long)(id + 1));
     unsigned long long best = 0;
     for (int r = 0; r < ranks; ++r) {
       const unsigned long long o = peer(r, 0);
@@ -636,8 +620,8 @@ __device__ void finish_list(Row<T>& r, const Weigher& weigh, const Cuts& q, int 
   Shared& sh = r.sh;
   constexpr int kEach = (WARP ? kWarpList : kList) / (WARP ? 32 : kThreads);
   const int tid = r.tid, lane = r.lane, first = tid * kEach;
-  auto total_of = [&](unsigned long long v) { return WARP ? warp_sum(v) : r.template block<false>(v); };
-  auto count_of = [&](uint32_t v) { return WARP ? __reduce_add_sync(kFull, v) : (uint32_t)r.template block<false>(v); };
+  auto total_of = [&](unsigned long long v) { return WARP ? warp_sum(v) : r.block_sum(v); };
+  auto count_of = [&](uint32_t v) { return WARP ? __reduce_add_sync(kFull, v) : (uint32_t)r.block_sum(v); };
   // thread i holds the ordered candidates kEach i .. kEach i + kEach - 1
   const int in_a = q.by_k ? min(listed, q.top_k) : listed;
   unsigned long long weight[kEach], sum = 0;
@@ -804,11 +788,11 @@ struct Bins {
   }
 };
 
-// Where the cuts lie in a histogram of counts, two bins per thread: starts[]
-// are its prefix sums; *last is the first bin that satisfies a cut (kCoarse - 1
-// when none does), *first a bin before top_p's border (or the k-th logit's).
-// `whole`: the sum of all weights, or 0 to take the bins' own estimate; slack:
-// how far beside its share top_p's border is looked for.
+// Where the cuts lie in a histogram of counts, two bins per thread (c0, c1):
+// starts[] are its prefix sums, *last the first bin by which every cut is met
+// (kCoarse when none is): top_k tokens; top_p's share of `whole`, the sum of
+// all weights, by the bins' least weights; or, without either, min_p's
+// floor_bin.  *crowded: a bin up to it has more than kCrowd tokens.
 template <typename T>
 __device__ __forceinline__ void find_cuts(Row<T>& r, const Bins& bins, uint32_t c0, uint32_t c1, const Cuts& q, float share,
                                           float whole, float floor_bin, uint32_t* last, bool* crowded) {
@@ -906,7 +890,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   if (nan) flag_status(p.status, kStatusNonFinite);
   uint32_t key_max = key_of(__fadd_rn(most, 0.0f)), key_low = ~key_of(least);
   r.block_max2(key_max, key_low);
-  r.publish(key_max, key_low, 0);
+  r.publish(key_max, key_low);
   for (int i = 0; i < ranks; ++i) {
     key_max = max(key_max, (uint32_t)r.peer(i, 0));
     key_low = max(key_low, (uint32_t)r.peer(i, 1));
@@ -929,7 +913,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
     });
     uint32_t inverse = kFull - id, none = 0;
     r.block_max2(inverse, none);
-    r.publish(inverse, 0, 0);
+    r.publish(inverse);
     if (rank == 0 && tid == 0) {
       for (int i = 0; i < ranks; ++i) inverse = max(inverse, (uint32_t)r.peer(i, 0));
       p.tokens[row] = (int32_t)(kFull - inverse);
@@ -962,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
           whole += w;
         }
       });
-      whole = r.template block<false>(whole);
+      whole = r.block_sum(whole);
     } else {
       r.each([&](float v, int) {
         const uint32_t b = bins.of(v);
@@ -970,7 +954,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       });
     }
     __syncthreads();
-    r.publish(whole, 0, 0);
+    r.publish(whole);
     uint32_t c0 = 0, c1 = 0;
     for (int i = 0; i < ranks; ++i) {
       const uint2 o = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&sh, i)->counts)[tid];
@@ -1032,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   // running > u * total  <=>  running > floor(u * total) for whole numbers
   unsigned long long target = (unsigned long long)floor(__dmul_rn(u, (double)total));
   if (target >= total) target = total - 1;
-  const int id = r.template locate<unsigned long long>(weight, before, before + sum, target);
+  const int id = r.locate(weight, before, before + sum, target);
   if (id >= 0 && tid == 0) {
     p.tokens[row] = id;
     const float v = r.at(id - base);
@@ -1046,7 +1030,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
 // rows than SMs spreads each over more.
 int cluster_of(int rows, int vocab) {
   int c = 1;
-  while (c < kMaxCluster && (vocab > c * 8192 || (rows * c * 2 <= 148 && vocab > c * 2048))) c *= 2;
+  while (c < kMaxCluster && (vocab > c * 8192 || (rows * c * 2 <= kSms && vocab > c * 2048))) c *= 2;
   return c;
 }
 
