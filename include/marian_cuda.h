@@ -343,7 +343,8 @@ typedef enum { MC_F32 = 0, MC_F16 = 1, MC_BF16 = 2 } mc_dtype;
  * (one token, one key/value head, key or value) is held as
  *   minimum = f16(min x),  scale = f16(f32(max x - minimum) * f32(1 / 15)),
  *   code    = clamp(round((x - minimum) / scale), 0, 15)   (ties to even;
- *             0 when scale is 0),
+ *             0 when scale is 0, or negative: a row whose minimum rounds
+ *             above its maximum),
  * and stands for minimum + scale * code.  A page holds page_tokens tokens of
  * every key/value head; for each head, in this order: the key rows' codes
  * [page_tokens][head_dim / 2] bytes (channel 2i in the low nibble of byte i,
@@ -355,7 +356,7 @@ typedef struct {
     const int32_t *page_table;   /* [batch][pages_per_seq] page ids */
     int64_t n_pages;
     int32_t page_tokens;         /* 8, 16 or 32 */
-    int32_t kv_heads;            /* >= 1 */
+    int32_t kv_heads;            /* 1..65536 */
     int32_t head_dim;            /* a multiple of 16, 16..128 */
     int32_t batch;               /* sequences, >= 0 */
     int32_t pages_per_seq;       /* >= 1; pages_per_seq * page_tokens < 2^31 */
@@ -396,7 +397,8 @@ mc_status mc_kv4_read(const mc_kv4_cache *cache, const mc_kv4_rows *rows, void *
  * them.  A query that sees nothing gets zeros and lse -inf.  lse (nullable,
  * [q_rows][heads]) receives ln sum_j w_j.  Rows outside every sequence are
  * left as they were; q ranges must not overlap.  16-bit types: the weights
- * are rounded to 11 bits before they meet the values; f32: to 22. */
+ * are rounded to 11 bits before they meet the values; f32: to 22.  A query
+ * with an infinity or a NaN gives NaN. */
 typedef struct {
     const void *q;               /* 16-byte aligned; strides as in mc_kv4_rows */
     void *out;                   /* may not overlap q */
@@ -430,9 +432,10 @@ mc_status mc_kv4_attention(const mc_kv4_cache *cache, const mc_kv4_attention_arg
  * zeros and lse -inf; lse (nullable, [q_rows][heads]) receives ln sum_j w_j.
  * Rows outside every sequence are left as they were; q ranges must not
  * overlap.  16-bit types: the weights are rounded to the type before they
- * meet the values; f32: products to 2^-21.  Infinities and NaN go the way of
- * f32 arithmetic: a key whose score is -inf has a weight of 0, an infinite
- * value gives an infinite output. */
+ * meet the values; f32: products to 2^-21, of numbers that are held to 2^-136
+ * where they are below 2^-114.  Infinities and NaN go the way of f32
+ * arithmetic: a key whose score is -inf has a weight of 0, an infinite value
+ * gives an infinite output. */
 typedef struct {
     const void *q, *k, *v;       /* 16-byte aligned; strides * element size multiples of 16 */
     void *out;                   /* may not overlap q, k or v */
@@ -445,7 +448,7 @@ typedef struct {
     int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride;
     int64_t v_row_stride, v_head_stride, out_row_stride, out_head_stride;
     int32_t dtype;               /* mc_dtype of q, k, v and out */
-    int32_t batch, heads, kv_heads;  /* heads a multiple of kv_heads */
+    int32_t batch, heads, kv_heads;  /* heads a multiple of kv_heads, <= 65536 */
     int32_t head_dim;            /* a multiple of 16, 16..128 */
     int32_t max_q_len, max_k_len;  /* no q_len[b] / k_len[b] is above them; max_k_len <= 2^31 - 256 */
     float scale;                 /* finite, below 2.35e38; commonly 1 / sqrt(head_dim) */

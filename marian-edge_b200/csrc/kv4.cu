@@ -291,8 +291,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const Kv4Pool 
 // subtraction, with no conversion.  Nibbles one place up give 16 (c - 8),
 // which q (a sixteenth of it) or the output takes back.
 //
-// q is scaled by a power of two to below 2^9 (exact for 16-bit types; f32 is
-// two f16 parts in the columns 0-3 and 4-7 of a tile, 22 bits).  The weights
+// q is scaled by a power of two to below 2^9 (exact for 16-bit types, but for
+// elements 2^20 and more below the row's largest; f32 is two f16 parts in the
+// columns 0-3 and 4-7 of a tile, 22 bits).  The weights
 // meet the values as w = p * scale_v in f16 (f32: two parts, again by
 // columns), so the running maximum is taken over x_j + exponent(scale_v_j),
 // which keeps w below 2^11 whatever the scales are; the sums of p and of
