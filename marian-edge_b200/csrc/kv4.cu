@@ -299,10 +299,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const Kv4Pool 
 // which keeps w below 2^11 whatever the scales are; the sums of p and of
 // p * middle_v are f32.
 //
-// Bound by the integer pipe where caches are long (62% busy: an AND-OR for two
+// Bound by the integer pipe where caches are long (64% busy: an AND-OR for two
 // operands, a byte permute for four) and by set-up and output where they are
 // short.  Measured: 8 x 65,536 keys, 8 heads of 128 with 4 queries each, bf16,
-// 183 us (3.1 TB/s of 4-bit rows; 201 us with four stages, whose memory leaves
+// 186 us (3.1 TB/s of 4-bit rows; 201 us with four stages, whose memory leaves
 // three CTAs per SM, 198 with five CTAs' registers); 1,024 single tokens over
 // 30 keys on average, 8 heads of 64, f32, 28 us.
 struct Kv4AttnParams {
